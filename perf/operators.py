@@ -1,0 +1,450 @@
+"""Timed cases of the 4-bit operators: MXFP4 quantization, the product with frozen MXFP4 weights, the gated
+feed-forward block over them, and distillation from a teacher's top logits.
+
+listed() names the cases, draw() makes more of the same ranges, prepare() makes what a program holds before the call,
+run() is one pass, in plain torch operations or, with own set, through the framework's entry points, work() counts what
+a pass cannot do without and exact() is the same result from the definition in 64 bits.
+"""
+import math
+import os
+import sys
+
+import torch
+
+own = False
+
+_PKG = os.path.join(os.getcwd(), "train-model-template_amd")
+
+
+def _ours():
+    if _PKG not in sys.path:
+        sys.path.insert(0, _PKG)
+    import distill
+    import mxfp4
+    return mxfp4, distill
+
+
+def listed():
+    return [
+        # a frozen projection quantized along both axes when a model is loaded, and its values read back
+        dict(name="quantize_weight_6144", kind="quantize", T=6144, K=2048, both=True, fmt="e2m1", dt="bf16"),
+        # an activation of a ragged length and a width that no block divides
+        dict(name="quantize_rows_1999", kind="quantize", T=1999, K=1000, both=False, fmt="e2m1", dt="f32"),
+        # a projection for one token while answering: the smallest call, latency and the weight's bytes
+        dict(name="linear_decode_1", kind="linear_decode", T=1, K=2048, N=6144, fmt="e4m3"),
+        # the same for a dozen conversations at once, down projection
+        dict(name="linear_decode_12", kind="linear_decode", T=12, K=6144, N=2048, fmt="e2m1"),
+        # attention projection in training, ragged micro-batch, forward and input gradient, 8-bit activations
+        dict(name="linear_step_1500", kind="linear_step", T=1500, K=2048, N=2048, fmt="e4m3"),
+        # the widest projection at the longest training length, everything in 4 bits
+        dict(name="linear_step_10752", kind="linear_step", T=10752, K=2048, N=6144, fmt="e2m1"),
+        # the feed-forward block for one token
+        dict(name="gated_decode_1", kind="gated_decode", T=1, K=2048, N=6144, fmt="e4m3", fn="silu"),
+        # its training step on a short, ragged micro-batch with adapters' output added to both projections
+        dict(name="gated_step_1000", kind="gated_step", T=1000, K=1024, N=3584, fmt="e4m3", fn="silu", add=True),
+        # its training step at the longest training length, 8-bit activations
+        dict(name="gated_step_10752", kind="gated_step", T=10752, K=2048, N=6144, fmt="e4m3", fn="silu", add=False),
+        # the loss alone on a few held-out positions
+        dict(name="distill_eval_16", kind="distill_eval", T=16, V=65536, k=64, tau=1.0, rest=False, dt="f32"),
+        # the loss and its gradient for one micro-batch, with the teacher's remaining mass in a bucket of its own
+        dict(name="distill_step_1000", kind="distill_step", T=1000, V=65536, k=32, tau=2.0, rest=True, dt="bf16"),
+        # the same over the unpruned vocabulary, an odd row length
+        dict(name="distill_step_2048", kind="distill_step", T=2048, V=248001, k=64, tau=1.0, rest=False, dt="bf16"),
+    ]
+
+
+def _log_int(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def _width(rng, lo, hi):
+    """A layer width: usually a multiple of 128, now and then of 8 or of nothing."""
+    n = _log_int(rng, lo, hi)
+    q = rng.choice([128, 128, 128, 8, 1])
+    return max(lo, n // q * q)
+
+
+def draw(rng):
+    kind = rng.choice(["quantize", "quantize", "linear_decode", "linear_decode", "linear_step", "linear_step",
+                       "gated_decode", "gated_step", "gated_step", "distill_eval", "distill_step", "distill_step"])
+    fmt = rng.choice(["e4m3", "e2m1"])
+    if kind == "quantize":
+        return dict(kind=kind, T=_log_int(rng, 1, 8000), K=_width(rng, 32, 6144), both=rng.random() < 0.5, fmt=fmt,
+                    dt=rng.choice(["bf16", "bf16", "f16", "f32"]))
+    if kind.startswith("distill"):
+        return dict(kind=kind, T=_log_int(rng, 1, 64 if kind == "distill_eval" else 2048), V=_log_int(rng, 1000, 248001),
+                    k=rng.choice([1, 8, 20, 32, 64, 100, 128]), tau=rng.choice([0.7, 1.0, 2.0, 4.0]),
+                    rest=rng.random() < 0.5, dt=rng.choice(["bf16", "bf16", "f16", "f32"]))
+    c = dict(kind=kind, T=_log_int(rng, 1, 16) if kind.endswith("decode") else _log_int(rng, 2, 10752),
+             K=_width(rng, 256, 2048 if kind.startswith("gated") else 6144), N=_width(rng, 256, 6144), fmt=fmt)
+    if c["K"] * c["N"] > 2048 * 6144:
+        c["K"] = 2048
+    if kind.startswith("gated"):
+        c["fn"] = rng.choice(["silu", "silu", "gelu"])
+    if kind == "gated_step":
+        c["add"] = rng.random() < 0.4
+    return c
+
+
+# ------------------------------------------------------------------------------------------------ inputs
+_DT = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+
+
+def _gen(seed, k):
+    return torch.Generator(device="cuda").manual_seed(1000003 * (seed + 1) + k)
+
+
+def _randn(seed, k, *shape, std=1.0):
+    return torch.randn(*shape, generator=_gen(seed, k), device="cuda") * std
+
+
+def _act(seed, k, rows, cols, std=1.0):
+    """Activations or upstream gradients: rows of different scale, a thousandth of the channels 30 times as large, as
+    the residual stream of a trained model has them."""
+    t = _randn(seed, k, rows, cols, std=std) * torch.exp(0.3 * _randn(seed, k + 500, rows, 1))
+    ch = torch.randperm(cols, generator=_gen(seed, k + 600), device="cuda")[:max(1, cols // 1000)]
+    t[:, ch] *= 30.0
+    return t
+
+
+def _inputs(case, seed):
+    kind = case["kind"]
+    if kind == "quantize":
+        return dict(x=_act(seed, 1, case["T"], case["K"], 0.02 if case["both"] else 1.0).to(_DT[case["dt"]]))
+    if kind.startswith("distill"):
+        T, V, k = case["T"], case["V"], case["k"]
+        # the teacher's top tokens of a position, all different, its logits there and the logsumexp over all it has
+        first = torch.randint(0, V, (T, 1), generator=_gen(seed, 1), device="cuda")
+        idx = (first + torch.arange(k, device="cuda") * max(1, V // (k + 1))) % V
+        t = torch.sort(_randn(seed, 2, T, k, std=2.0) + 6.0, dim=1, descending=True).values
+        z = _randn(seed, 3, T, V, std=1.5)
+        z.scatter_(1, idx, t + _randn(seed, 4, T, k))
+        d = dict(z=z.to(_DT[case["dt"]]), idx=idx.to(torch.int32), t=t,
+                 w=torch.full((T,), 1.0 / T, device="cuda"))
+        if case["rest"]:
+            d["lse"] = torch.logsumexp(t / case["tau"], 1) + 0.05 + 0.2 * torch.rand(
+                T, generator=_gen(seed, 5), device="cuda")
+        if T > 8:  # positions that are not trained on
+            d["idx"][T // 3] = -1
+        return d
+    T, K, N = case["T"], case["K"], case["N"]
+    bf = torch.bfloat16
+    d = dict(x=_act(seed, 1, T, K).to(bf))
+    if kind.startswith("linear"):
+        d["w"] = _randn(seed, 2, N, K, std=0.02).to(bf)
+    else:
+        d["wg"], d["wu"] = (_randn(seed, k, N, K, std=0.02).to(bf) for k in (2, 3))
+    if kind.endswith("step"):
+        d["dy"] = _act(seed, 4, T, N, 1e-2).to(bf)
+    if case.get("add"):
+        d["add"] = _randn(seed, 5, T, 2 * N, std=0.1).to(bf)
+    return d
+
+
+# ------------------------------------------------------------------------------------------------ plain forms
+def _blocks(x):
+    """[R, C] -> [R, ceil(C / 32), 32], zeros past C."""
+    pad = -x.shape[1] % 32
+    return torch.nn.functional.pad(x, (0, pad)).reshape(x.shape[0], -1, 32)
+
+
+def _pow2(e, dtype):
+    """2 ^ e, exactly (e whole, within the type's normal numbers; -127 as well in 32 bits)."""
+    if dtype == torch.float64:
+        return ((e.to(torch.int64) + 1023) << 52).view(torch.float64)
+    e = e.to(torch.int32)
+    return torch.where(e > -127, (e + 127) << 23, 1 << 22).view(torch.float32)
+
+
+def _exponent(amax, top):
+    """The least e >= -127 with amax <= top * 2^e, top = (m_top) 2^(e_top)."""
+    m, e = torch.frexp(amax)
+    mt, et = math.frexp(top)
+    e = torch.where(m > mt, e - et + 1, e - et)
+    return torch.where(amax > 0, e, -127).clamp(min=-127)
+
+
+def _round_values(r, fmt):
+    """r rounded to the format's values, ties to even; r within the format's range."""
+    a = r.abs()
+    if fmt == "e2m1":
+        step = torch.where(a < 2, 0.5, torch.where(a < 4, 1.0, 2.0))
+    else:
+        _, e = torch.frexp(a)
+        step = _pow2((e - 4).clamp(min=-9), a.dtype)
+    return torch.round(r / step) * step
+
+
+_TOP = {"e2m1": 6.0, "e4m3": 448.0}
+
+
+def _mx(x, fmt):
+    """The values that the MX form of x [R, C] stands for, in 32 bits."""
+    b = _blocks(x.float())
+    e = _exponent(b.abs().amax(2, keepdim=True), _TOP[fmt])
+    v = _round_values(b * _pow2(-e, b.dtype), fmt) * _pow2(e, b.dtype)
+    return v.reshape(x.shape[0], -1)[:, :x.shape[1]]
+
+
+_E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+def _pack(w):
+    """A weight [N, K] as a program without an own layout keeps it: two 4-bit codes a byte, one exponent a block."""
+    b = _blocks(w.float())
+    e = _exponent(b.abs().amax(2, keepdim=True), 6.0)
+    v = _round_values(b * _pow2(-e, b.dtype), "e2m1")
+    code = torch.bucketize(v.abs(), torch.tensor(_E2M1, device=w.device)) + 8 * (v < 0)
+    code = code.reshape(w.shape[0], -1).to(torch.uint8)
+    return code[:, 0::2] | (code[:, 1::2] << 4), (e[:, :, 0] + 127).to(torch.uint8), w.shape[1]
+
+
+def _unpack(p):
+    code, e, K = p
+    table = torch.tensor(_E2M1 + tuple(-v for v in _E2M1), device=code.device)
+    v = table[torch.stack([code & 15, code >> 4], 2).reshape(code.shape[0], -1, 32).int()]
+    v = v * _pow2(e.int()[:, :, None] - 127, v.dtype)
+    return v.reshape(code.shape[0], -1)[:, :K]
+
+
+def _gate(fn, g):
+    """fn(g) and its derivative."""
+    if fn == "silu":
+        s = torch.sigmoid(g)
+        return g * s, s * (1 + g * (1 - s))
+    c = math.sqrt(2 / math.pi)
+    t = torch.tanh(c * (g + 0.044715 * g ** 3))
+    return 0.5 * g * (1 + t), 0.5 * (1 + t) + 0.5 * g * (1 - t * t) * c * (1 + 3 * 0.044715 * g * g)
+
+
+def _plain_distill(case, d, grad):
+    tau, V = case["tau"], case["V"]
+    z = d["z"].float() / tau
+    live = (d["idx"] >= 0).any(1)
+    idx = d["idx"].clamp(min=0).long()
+    t = d["t"] / tau
+    top = z.amax(1, keepdim=True)
+    ez = torch.exp(z - top)
+    total = ez.sum(1, keepdim=True)
+    if case["rest"]:
+        p = torch.exp(t - d["lse"][:, None])
+        rest = (1 - p.sum(1, keepdim=True)).clamp(min=0)
+    else:
+        p = torch.exp(t - t.amax(1, keepdim=True))
+        p = p / p.sum(1, keepdim=True)
+        rest = torch.zeros_like(total)
+    logq = z.gather(1, idx) - top - torch.log(total)
+    loss = (p * (torch.log(p) - logq)).sum(1, keepdim=True)
+    other = ez.scatter(1, idx, torch.zeros_like(p)).sum(1, keepdim=True)
+    if case["rest"]:
+        part = rest * (torch.log(rest) - torch.log(other / total))
+        loss = loss + torch.where(rest > 0, part, torch.zeros_like(part))
+    loss = torch.where(live, loss[:, 0] * tau * tau, torch.zeros_like(loss[:, 0]))
+    if not grad:
+        return loss
+    scale = (d["w"] * tau * live)[:, None]
+    g = ez * ((1 / total - rest / other if case["rest"] else 1 / total) * scale)
+    g.scatter_(1, idx, torch.where(live[:, None], (torch.exp(logq) - p) * scale, g.gather(1, idx)))
+    return loss, g.to(d["z"].dtype)
+
+
+def _plain(st):
+    case, d = st["case"], st["d"]
+    kind = case["kind"]
+    if kind == "quantize":
+        x = d["x"]
+        bf = torch.bfloat16
+        v = _mx(x, case["fmt"]).to(bf)
+        return (v, _mx(x.t(), case["fmt"]).to(bf)) if case["both"] else v
+    if kind.startswith("distill"):
+        return _plain_distill(case, d, kind == "distill_step")
+    x, dt, fmt, N = d["x"], d["x"].dtype, case["fmt"], case["N"]
+    acc = _mx(x, fmt) @ _unpack(st["w"]).t()
+    if kind == "linear_decode":
+        return acc.to(dt)
+    if kind == "linear_step":
+        return acc.to(dt), (_mx(d["dy"], fmt) @ _unpack(st["wt"]).t()).to(dt)
+    if case.get("add"):
+        acc = acc + d["add"].float()
+    h = (_gate(case["fn"], acc[:, :N])[0] * acc[:, N:]).to(dt)
+    if kind == "gated_decode":
+        return h
+    kept = acc.to(dt).float()  # what is kept for the backward pass has the activations' type, by definition
+    f, df = _gate(case["fn"], kept[:, :N])
+    dy = d["dy"].float()
+    dgu = torch.cat([dy * kept[:, N:] * df, dy * f], 1)
+    dx = (_mx(dgu, fmt) @ _unpack(st["wt"]).t()).to(dt)
+    return (h, dx, dgu.to(dt)) if case.get("add") else (h, dx)
+
+
+# ------------------------------------------------------------------------------------------------ the passes
+def prepare(case, seed):
+    """Inputs, and the frozen weight in the form that a program keeps from one pass to the next."""
+    d = _inputs(case, seed)
+    st = dict(case=case, d=d)
+    kind = case["kind"]
+    if kind.startswith("linear") or kind.startswith("gated"):
+        linear = kind.startswith("linear")
+        if own:
+            mxfp4, _ = _ours()
+            st["w"] = mxfp4.Weight(d.pop("w")) if linear else mxfp4.GatedWeight(d.pop("wg"), d.pop("wu"))
+        else:
+            w = d.pop("w") if linear else torch.cat([d.pop("wg"), d.pop("wu")])
+            st["w"] = _pack(w)
+            if kind.endswith("step"):
+                st["wt"] = _pack(w.t())
+        if kind.endswith("step"):
+            d["x"].requires_grad_(True)
+            if "add" in d:
+                d["add"].requires_grad_(True)
+    return st
+
+
+def _own(st):
+    mxfp4, distill = _ours()
+    case, d = st["case"], st["d"]
+    kind = case["kind"]
+    if kind == "quantize":
+        m = mxfp4.mx4_quant(d["x"], fmt=case["fmt"], both=case["both"])
+        if case["both"]:
+            return tuple(mxfp4.mx4_dequant(a, torch.bfloat16) for a in m)
+        return mxfp4.mx4_dequant(m, torch.bfloat16)
+    if kind == "distill_eval":
+        return distill.topk_kl(d["z"], d["idx"], d["t"], temperature=case["tau"], teacher_lse=d.get("lse"))
+    if kind == "distill_step":
+        return distill.topk_kl_rows(d["z"], d["idx"], d["t"], d["w"], temperature=case["tau"], teacher_lse=d.get("lse"))
+    if kind == "linear_decode":
+        return mxfp4.mx4_linear(d["x"], st["w"], act=case["fmt"])
+    if kind == "linear_step":
+        y = mxfp4.mx4_linear(d["x"], st["w"], act=case["fmt"])
+        return (y.detach(),) + torch.autograd.grad(y, d["x"], d["dy"])
+    if kind == "gated_decode":
+        return mxfp4.mx4_gated(d["x"], st["w"], fn=case["fn"], act=case["fmt"])
+    h = mxfp4.mx4_gated(d["x"], st["w"], add=d.get("add"), fn=case["fn"], act=case["fmt"])
+    leaves = (d["x"], d["add"]) if "add" in d else (d["x"],)
+    return (h.detach(),) + torch.autograd.grad(h, leaves, d["dy"])
+
+
+def run(state):
+    if own:
+        return _own(state)
+    with torch.no_grad():
+        return _plain(state)
+
+
+def work(case):
+    kind, T = case["kind"], case["T"]
+    size = {"bf16": 2, "f16": 2, "f32": 4}.get(case.get("dt"), 2)
+    if kind == "quantize":
+        n = T * case["K"]
+        code = (17 if case["fmt"] == "e2m1" else 33) / 32
+        axes = 2 if case["both"] else 1
+        return {"bytes": n * size + axes * n * (code + 2), "flops": 2 * axes * n}
+    if kind.startswith("distill"):
+        n = T * case["V"]
+        step = kind == "distill_step"
+        return {"bytes": n * size * (2 if step else 1) + T * case["k"] * 8 + 8 * T, "flops": n * (8 if step else 4)}
+    K, N = case["K"], case["N"]
+    step = kind.endswith("step")
+    if kind.startswith("linear"):
+        return {"bytes": (T * (K + N) * 2 + N * K * 17 / 32) * (2 if step else 1),
+                "flops": 2 * T * N * K * (2 if step else 1)}
+    by = T * (K + N) * 2 + 2 * N * K * 17 / 32
+    if step:
+        by = 2 * by + (T * 2 * N * 2 * 2 if case["add"] else 0)
+    return {"bytes": by, "flops": 4 * T * N * K * (2 if step else 1)}
+
+
+# ------------------------------------------------------------------------------------------------ 64 bits
+def _values64(fmt):
+    if fmt == "e2m1":
+        return torch.tensor(_E2M1, dtype=torch.float64, device="cuda")
+    v = [m * 2.0 ** -9 for m in range(8)]
+    v += [(8 + m) * 2.0 ** (e - 10) for e in range(1, 16) for m in range(8)]
+    return torch.tensor(v[:-1], dtype=torch.float64, device="cuda")
+
+
+def _mx64(x, fmt):
+    """MX values of x by looking for the nearest of the format's values, of two equally near ones that with an even
+    code; rows in pieces, to bound the memory."""
+    vals = _values64(fmt)
+    mid = (vals[1:] + vals[:-1]) / 2
+    out = torch.empty(x.shape, dtype=torch.float64, device=x.device)
+    for r in range(0, x.shape[0], 2048):
+        b = _blocks(x[r:r + 2048].double())
+        amax = b.abs().amax(2, keepdim=True)
+        e = torch.ceil(torch.log2(torch.where(amax > 0, amax, torch.ones_like(amax)) / vals[-1]))
+        e = torch.where(vals[-1] * _pow2(e - 1, b.dtype) >= amax, e - 1, e)  # log2 near a whole number
+        e = torch.where(vals[-1] * _pow2(e, b.dtype) < amax, e + 1, e)
+        e = torch.where(amax > 0, e, torch.full_like(e, -127.0)).clamp(min=-127.0)
+        a = b.abs() * _pow2(-e, b.dtype)
+        lo = torch.searchsorted(mid, a)                  # ties to the lower code
+        hi = torch.searchsorted(mid, a, right=True)      # ties to the upper code
+        code = torch.where((lo != hi) & (lo % 2 == 1), hi, lo)
+        v = torch.copysign(vals[code], b) * _pow2(e, b.dtype)
+        out[r:r + 2048] = v.reshape(v.shape[0], -1)[:, :x.shape[1]]
+    return out
+
+
+def _fn64(fn, g):
+    with torch.enable_grad():
+        g = g.detach().requires_grad_(True)
+        f = g / (1 + torch.exp(-g)) if fn == "silu" else 0.5 * g * (
+            1 + torch.tanh(math.sqrt(2 / math.pi) * (g + 0.044715 * g * g * g)))
+        return f.detach(), torch.autograd.grad(f.sum(), g)[0]
+
+
+def _distill64(case, d):
+    tau, losses, grads = case["tau"], [], []
+    for r in range(0, case["T"], 256):
+        z = d["z"][r:r + 256].double() / tau
+        idx, t, w = d["idx"][r:r + 256].long(), d["t"][r:r + 256].double() / tau, d["w"][r:r + 256].double()
+        live = idx[:, 0] >= 0
+        idx = idx.clamp(min=0)
+        logq = torch.log_softmax(z, 1)
+        logp = t - d["lse"][r:r + 256].double()[:, None] if case["rest"] else torch.log_softmax(t, 1)
+        p = logp.exp()
+        loss = (p * (logp - logq.gather(1, idx))).sum(1)
+        q = logq.exp()
+        if case["rest"]:
+            pr = 1 - p.sum(1)
+            lr = torch.logsumexp(logq.scatter(1, idx, torch.full_like(p, -math.inf)), 1)
+            loss = loss + torch.where(pr > 0, pr * (pr.clamp(min=1e-300).log() - lr), torch.zeros_like(pr))
+            g = q * (1 - (pr.clamp(min=0).log() - lr).exp())[:, None]
+        else:
+            g = q.clone()
+        g.scatter_(1, idx, q.gather(1, idx) - p)
+        losses.append(torch.where(live, loss * tau * tau, torch.zeros_like(loss)))
+        if case["kind"] == "distill_step":
+            grads.append(g * (tau * w * live)[:, None])
+    loss = torch.cat(losses)
+    return (loss, torch.cat(grads)) if grads else loss
+
+
+def exact(case, seed):
+    with torch.no_grad():
+        d = _inputs(case, seed)
+        kind, fmt = case["kind"], case.get("fmt")
+        if kind == "quantize":
+            v = _mx64(d["x"], fmt)
+            return (v, _mx64(d["x"].t(), fmt)) if case["both"] else v
+        if kind.startswith("distill"):
+            return _distill64(case, d)
+        w = d["w"] if kind.startswith("linear") else torch.cat([d["wg"], d["wu"]])
+        acc = _mx64(d["x"], fmt) @ _mx64(w, "e2m1").t()
+        if kind == "linear_decode":
+            return acc
+        if kind == "linear_step":
+            return acc, _mx64(d["dy"], fmt) @ _mx64(w.t(), "e2m1").t()
+        N = case["N"]
+        if case.get("add"):
+            acc = acc + d["add"].double()
+        h = _fn64(case["fn"], acc[:, :N])[0] * acc[:, N:]
+        if kind == "gated_decode":
+            return h
+        kept = acc.float().to(d["x"].dtype).double()
+        f, df = _fn64(case["fn"], kept[:, :N])
+        dy = d["dy"].double()
+        dgu = torch.cat([dy * kept[:, N:] * df, dy * f], 1)
+        dx = _mx64(dgu, fmt) @ _mx64(w.t(), "e2m1").t()
+        return (h, dx, dgu) if case.get("add") else (h, dx)
