@@ -272,9 +272,9 @@ def _plain(st):
     kept = acc.to(dt).float()  # what is kept for the backward pass has the activations' type, by definition
     f, df = _gate(case["fn"], kept[:, :N])
     dy = d["dy"].float()
-    dgu = torch.cat([dy * kept[:, N:] * df, dy * f], 1)
-    dx = (_mx(dgu, fmt) @ _unpack(st["wt"]).t()).to(dt)
-    return (h, dx, dgu.to(dt)) if case.get("add") else (h, dx)
+    dg, du = dy * kept[:, N:] * df, dy * f
+    dx = (_mx(dg, fmt) @ _unpack(st["wt"][0]).t() + _mx(du, fmt) @ _unpack(st["wt"][1]).t()).to(dt)
+    return (h, dx, torch.cat([dg, du], 1).to(dt)) if case.get("add") else (h, dx)
 
 
 # ------------------------------------------------------------------------------------------------ the passes
@@ -289,10 +289,10 @@ def prepare(case, seed):
             mxfp4, _ = _ours()
             st["w"] = mxfp4.Weight(d.pop("w")) if linear else mxfp4.GatedWeight(d.pop("wg"), d.pop("wu"))
         else:
-            w = d.pop("w") if linear else torch.cat([d.pop("wg"), d.pop("wu")])
-            st["w"] = _pack(w)
+            w = (d.pop("w"),) if linear else (d.pop("wg"), d.pop("wu"))
+            st["w"] = _pack(torch.cat(w))
             if kind.endswith("step"):
-                st["wt"] = _pack(w.t())
+                st["wt"] = _pack(w[0].t()) if linear else tuple(_pack(a.t()) for a in w)
         if kind.endswith("step"):
             d["x"].requires_grad_(True)
             if "add" in d:
@@ -445,6 +445,6 @@ def exact(case, seed):
         kept = acc.float().to(d["x"].dtype).double()
         f, df = _fn64(case["fn"], kept[:, :N])
         dy = d["dy"].double()
-        dgu = torch.cat([dy * kept[:, N:] * df, dy * f], 1)
-        dx = _mx64(dgu, fmt) @ _mx64(w.t(), "e2m1").t()
-        return (h, dx, dgu) if case.get("add") else (h, dx)
+        dg, du = dy * kept[:, N:] * df, dy * f
+        dx = _mx64(dg, fmt) @ _mx64(d["wg"].t(), "e2m1").t() + _mx64(du, fmt) @ _mx64(d["wu"].t(), "e2m1").t()
+        return (h, dx, torch.cat([dg, du], 1)) if case.get("add") else (h, dx)
