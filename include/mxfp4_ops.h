@@ -1,0 +1,113 @@
+/* C-ABI of the 4-bit operators in libmxfp8_mlp.so (gfx950): MXFP4 quantization, products with MXFP4 weights, the
+ * gated feed-forward block over them, and distillation from a teacher's top logits.
+ *
+ * Every entry point takes device pointers, sizes and a hipStream_t (as void*), allocates nothing and does not wait.  It
+ * returns 0, MXFP8_ERR_ARG (-1) or a HIP error code; mxfp8_last_error() (mxfp8_mlp.h) has the message.
+ *
+ * MX operand [R, C]: codes along C in blocks of 32 with one E8M0 scale each, both in blocked layouts.
+ *   C is padded with zeros to Cp = ceil(C / 128) * 128; rows are padded to Rp = ceil(R / 32) * 32 (contents of the padded
+ *   rows are undefined).
+ *   E2M1 codes: blocks of 16 rows x 128 codes, 1 KB each, block (r / 16, c / 128) at ((r / 16) * (Cp / 128) + c / 128) *
+ *     1024; in a block row r % 16 takes 64 bytes whose 16-byte chunk k (codes 32 k ..) sits at position k ^ ((r >> 2) & 3);
+ *     the code of an even column is the low half of its byte.  Rp * Cp / 2 bytes.
+ *   E4M3 codes: the MX-tiled layout of mxfp8_mlp.h (blocks of 16 rows x 64 codes).  Rp * Cp bytes.
+ *   Scales: the 128x4 blocked layout of mxfp8_mlp.h, ceil(R / 128) * (Cp / 128) * 512 bytes.
+ * Row orders of a weight operand: MXFP4_ROWS_PLAIN; MXFP4_ROWS_PI: inside each 32-row block position a holds row
+ * ((a >> 2) & 1) * 16 + (a >> 3) * 4 + (a & 3), which gives every lane of the GEMM's epilogue 16 contiguous columns;
+ * MXFP4_ROWS_GATE / _UP: the PI order, with gate block j at block 2 j and up block j at 2 j + 1 of one shared operand.
+ */
+#ifndef MXFP4_OPS_H
+#define MXFP4_OPS_H
+
+#include <stdint.h>
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+#define MXFP4_OPS_ABI_VERSION 1
+
+/* element types of plain tensors */
+#define MXFP4_BF16 0
+#define MXFP4_F16 1
+#define MXFP4_F32 2
+/* code formats */
+#define MXFP4_E2M1 4
+#define MXFP4_E4M3 8
+/* row orders */
+#define MXFP4_ROWS_PLAIN 0
+#define MXFP4_ROWS_PI 1
+#define MXFP4_ROWS_GATE 2
+#define MXFP4_ROWS_UP 3
+/* gate functions */
+#define MXFP4_SILU 0
+#define MXFP4_GELU 1 /* the tanh form */
+
+int mxfp4_abi_version(void);
+
+/* x [rows, cols] (type, row stride ld_x in elements, unit column stride) -> codes and scales.
+ * q, s: the operand along the columns, fmt, row order `order`, or both null.
+ * qt, st: the operand of x's transpose [cols, rows], row order order_t, or both null.  Its columns start at column tile
+ * t_tile0 (128 wide) of an operand with t_tiles column tiles (one weight: 0 and ceil(rows / 128)). */
+int mxfp4_quant(const void* x, int64_t type, int64_t rows, int64_t cols, int64_t ld_x, int64_t fmt, void* q, void* s,
+                int64_t order, void* qt, void* st, int64_t order_t, int64_t t_tile0, int64_t t_tiles, void* stream);
+
+/* The values of an operand in the PLAIN order: out [rows, cols] contiguous, of the given type (exact in every type that
+ * holds the exponent). */
+int mxfp4_dequant(const void* q, const void* s, int64_t rows, int64_t cols, int64_t fmt, void* out, int64_t type,
+                  void* stream);
+
+/* C [M, N] (type, row stride ldc) = A [M, K] . B [N, K]^T: A E4M3 or E2M1 (a_fmt) in the PLAIN order, B E2M1 in the PLAIN
+ * or PI order, K the padded width (a multiple of 128) of both; fp32 sums, one rounding. */
+int mxfp4_gemm(const void* a, const void* sa, int64_t a_fmt, const void* b, const void* sb, int64_t b_order, int64_t M,
+               int64_t N, int64_t K, void* c, int64_t ldc, int64_t type, void* stream);
+
+/* The gated block: [g | u] = A . [W_gate; W_up]^T (+ add), h [M, N] = fn(g) * u.  B holds gate and up in the GATE and UP
+ * orders.  add: [M, 2 N] of the type with row stride ld_add (0 repeats one row) or null.  gu: null, or
+ * mxfp4_gated_saved_elems(M, N) elements of the type for the backward pass.  type bf16 or f16. */
+int mxfp4_gated(const void* a, const void* sa, int64_t a_fmt, const void* b, const void* sb, int64_t M, int64_t N,
+                int64_t K, const void* add, int64_t ld_add, int64_t fn, void* h, int64_t ldh, void* gu, int64_t type,
+                void* stream);
+int64_t mxfp4_gated_saved_elems(int64_t M, int64_t N);
+
+/* Backward of the gate: dh [M, N] (row stride ld_dh) and the saved gu -> the operand of [dg | du] (fmt, PLAIN order): dg in
+ * columns 0 .. N - 1, du from column ceil(N / 128) * 128 on, so 2 * ceil(N / 128) * 128 columns in all; and dgu [M, 2 N]
+ * contiguous of the type, or null. */
+int mxfp4_gated_bwd(const void* gu, const void* dh, int64_t ld_dh, int64_t M, int64_t N, int64_t fn, int64_t type,
+                    int64_t fmt, void* q, void* s, void* dgu, void* stream);
+
+/* Few rows (M <= MXFP4_FEW_ROWS): the quantization of x [M, K] (type bf16 or f16, row stride ld_x, fmt) and the product in
+ * one launch; results as mxfp4_quant followed by mxfp4_gemm / mxfp4_gated, up to the order of the fp32 sums. */
+#define MXFP4_FEW_ROWS 16
+int mxfp4_few(const void* x, int64_t ld_x, int64_t fmt, const void* b, const void* sb, int64_t M, int64_t N, int64_t K,
+              void* c, int64_t ldc, int64_t type, void* stream);
+int mxfp4_few_gated(const void* x, int64_t ld_x, int64_t fmt, const void* b, const void* sb, int64_t M, int64_t N,
+                    int64_t K, const void* add, int64_t ld_add, int64_t fn, void* h, int64_t ldh, int64_t type,
+                    void* stream);
+
+/* Distillation from a teacher's top logits, row by row: with p the teacher's distribution over its k entries and q =
+ * softmax(logits / tau),
+ *   loss = tau^2 (sum p (log p - log q) + p_rest (log p_rest - log q_rest)),  grad = weight * d loss / d logits.
+ * logits [T, V] (type, row stride ld); idx [T, k] (idx_bytes 4 or 8, row stride ld_idx), entries outside [0, V) are padding;
+ * t [T, k] fp32 (row stride ld_t).  lse null: p = softmax(t / tau) over the entries, p_rest = 0; else [T] fp32, the
+ * teacher's logsumexp of all its logits / tau: p = exp(t / tau - lse), p_rest = max(0, 1 - sum p).
+ * loss [T] fp32 or null; grad [T, V] of the logits' type (row stride ld_grad; may be the logits themselves) or null, with
+ * weight [T] fp32 (null: 1).  Rows without a teacher entry of positive mass, and the gradient of rows of weight 0, are 0
+ * whatever the logits hold.
+ * parts: pieces a row is split into.  1: one launch, ws unused.  More: two launches that pass distill_workspace_size bytes
+ * in ws.  stages: 3 both; 1 only the statistics into ws; 2 only the loss and gradient from them (parts > 1, or ws kept). */
+#define DISTILL_STATS 1
+#define DISTILL_FINISH 2
+#define DISTILL_MAX_K 1024
+#define DISTILL_MAX_PARTS 256
+int64_t distill_parts(int64_t T, int64_t V, int64_t rest);
+int64_t distill_workspace_size(int64_t T, int64_t k, int64_t parts);
+int distill_topk_kl(const void* logits, int64_t type, int64_t ld, int64_t T, int64_t V, const void* idx, int64_t idx_bytes,
+                    int64_t ld_idx, const float* t, int64_t ld_t, int64_t k, float tau, const float* lse,
+                    const float* weight, float* loss, void* grad, int64_t ld_grad, int64_t parts, int64_t stages, void* ws,
+                    void* stream);
+
+#ifdef __cplusplus
+}
+#endif
+#endif

@@ -126,6 +126,28 @@ def host():
     return _host
 
 
+HOST4_PATH = os.path.join(_HERE, "_mx4host.so")
+OPS_ABI_VERSION = 1  # include/mxfp4_ops.h
+_host4 = None
+
+
+def host4():
+    """The native host module of the 4-bit operators and the distillation loss (csrc/host4.cpp)."""
+    global _host4
+    if _host4 is None:
+        lib = load()
+        if not os.path.exists(HOST4_PATH):
+            raise NativeError(f"{HOST4_PATH} is not built: run `python -c 'import __graft_entry__ as g; g.build()'`")
+        spec = importlib.util.spec_from_file_location("_mx4host", HOST4_PATH)
+        m = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(m)
+        if not m.abi_version() == lib.mxfp4_abi_version() == OPS_ABI_VERSION:
+            raise NativeError(f"{HOST4_PATH}: built against another version of the library; rebuild both")
+        m.set_error(NativeError)
+        _host4 = m
+    return _host4
+
+
 _raw_stream = torch._C._cuda_getCurrentRawStream  # device index -> the current HIP stream, as an int
 
 

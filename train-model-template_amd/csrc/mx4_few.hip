@@ -1,0 +1,259 @@
+// The products of mx4_gemm.hip for at most 16 rows (single tokens, a few conversations): the quantization of x, the
+// product and the gate in one launch.
+//
+// What bounds it: the weight's bytes, read once (17/32 a code), and, for one token, the latency of one launch and of two
+// dependent loads.  A workgroup takes 16 weight rows (gate and up: 16 of each); its waves split K and add their sums
+// through LDS.  One v_mfma_scale_f32_16x16x128 takes a 1 KB weight block as it lies in memory, 16 bytes a lane, with the
+// tokens as the other operand's rows; rows past M repeat the last one.  Its operand of x needs no exchange in E2M1 (lane l
+// holds a whole 32-block of token l % 16) and two lane swaps in E4M3 (each block lies in two lanes), so every wave
+// quantizes what it multiplies, from registers, while its weight blocks are under way.
+#include "abi_common.h"
+#include "mx4_device.h"
+
+using namespace mx4;
+
+namespace {
+
+constexpr int kU = 4;  // K tiles in flight in a wave
+
+struct FewArgs {
+  const void* x;
+  int64_t ld_x;
+  const uint8_t* b;
+  const uint8_t* sb;
+  int M, N, K, kt;  // K: columns of x; kt: K tiles of 128 of B
+  void* c;
+  int64_t ldc;
+  const void* add;
+  int64_t ld_add;
+  int fn, vec_x, vec_c;
+};
+
+// 16 values (packed pairs) of columns k.. of a row; zeros past K
+template <int kT>
+__device__ __forceinline__ void load16p(const uint16_t* row, int k, int K, bool vec, uint32_t* w) {
+  if (vec && k + 16 <= K) {
+    const uint4 a = *reinterpret_cast<const uint4*>(row + k), b = *reinterpret_cast<const uint4*>(row + k + 8);
+    w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+    w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t lo = k + 2 * i < K ? row[k + 2 * i] : 0, up = k + 2 * i + 1 < K ? row[k + 2 * i + 1] : 0;
+      w[i] = lo | (up << 16);
+    }
+  }
+}
+
+// magnitude bits of the largest of 16 packed values, as of an fp32 value (16-bit patterns order like magnitudes)
+template <int kT>
+__device__ __forceinline__ uint32_t absmax16p(const uint32_t* w) {
+  u16x2 m = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = absmax2(m, w[i]);
+  const uint32_t b = max(m.x, m.y);
+  if constexpr (kT == MXFP4_BF16) return b << 16;
+  return abs_bits((float)__builtin_bit_cast(_Float16, (uint16_t)b));
+}
+
+template <int kT>
+__device__ __forceinline__ void unpack16(const uint32_t* w, float* v) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if constexpr (kT == MXFP4_BF16) {
+      v[2 * i] = bf16_lo(w[i]);
+      v[2 * i + 1] = bf16_hi(w[i]);
+    } else {
+      const f16x2 h = __builtin_bit_cast(f16x2, w[i]);
+      v[2 * i] = (float)h[0];
+      v[2 * i + 1] = (float)h[1];
+    }
+  }
+}
+
+// The lane's operand of one K tile from its 32 values w (E2M1: columns 32 g ..; E4M3: 16 g .. and 64 + 16 g ..), and the
+// scale byte that the instruction reads from this lane (32-block g of its token)
+template <int kT, int kFmt>
+__device__ __forceinline__ v8i operand(const uint32_t* w, int g, uint32_t& scale) {
+  uint32_t a0 = absmax16p<kT>(w), a1 = absmax16p<kT>(w + 8), p, q, e0, e1;
+  if constexpr (kFmt == MXFP4_E4M3) {
+    pair16(a0, p, q);
+    e0 = block_exponent<kFmt>(max(p, q));  // block g / 2
+    pair16(a1, p, q);
+    e1 = block_exponent<kFmt>(max(p, q));  // block 2 + g / 2
+    const uint32_t mine = e0 | (e1 << 8);
+    pair32(mine, p, q);
+    const uint32_t other = p ^ q ^ mine;  // lane l ^ 32: blocks of g ^ 2
+    scale = g == 0 ? e0 : g == 1 ? other & 255u : g == 2 ? other >> 8 : e1;
+  } else {
+    e0 = e1 = scale = block_exponent<kFmt>(max(a0, a1));
+  }
+  float v[16];
+  v8i r = {0, 0, 0, 0, 0, 0, 0, 0};
+  uint32_t c[2], d[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    unpack16<kT>(w + 8 * h, v);
+    encode8<kFmt>(v, h ? e1 : e0, c);
+    encode8<kFmt>(v + 8, h ? e1 : e0, d);
+    if constexpr (kFmt == MXFP4_E4M3) {
+      r[4 * h] = (int)c[0];
+      r[4 * h + 1] = (int)c[1];
+      r[4 * h + 2] = (int)d[0];
+      r[4 * h + 3] = (int)d[1];
+    } else {
+      r[2 * h] = (int)c[0];
+      r[2 * h + 1] = (int)d[0];
+    }
+  }
+  return r;
+}
+
+template <int kT, int kFmt, bool kGated, int kWaves>
+__global__ __launch_bounds__(64 * kWaves) void few_kernel(const FewArgs a) {
+  typedef typename Elem<kT>::T T;
+  constexpr int kB = kGated ? 2 : 1;
+  __shared__ __attribute__((aligned(16))) f32x4 part[kWaves][kB][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r16 = lane & 15, g = lane >> 4;
+  // the weight rows: 16-row block `blockIdx.x` of B, or half h of gate block and up block j
+  const int64_t blk = blockIdx.x;
+  int64_t rb[kB];  // first row of the 16
+  if constexpr (kGated) {
+    rb[0] = (blk >> 1) * 64 + (blk & 1) * 16;
+    rb[1] = rb[0] + 32;
+  } else {
+    rb[0] = blk * 16;
+  }
+  const int per = (a.kt + kWaves - 1) / kWaves, t0 = wave * per, t1 = min(a.kt, t0 + per);
+  const uint8_t* wp[kB];
+  const uint8_t* sp[kB];
+#pragma unroll
+  for (int i = 0; i < kB; ++i) {
+    wp[i] = a.b + (rb[i] >> 4) * a.kt * 1024 + r16 * 64 + ((g ^ ((r16 >> 2) & 3)) << 4);
+    const int64_t r = rb[i] + r16;
+    sp[i] = a.sb + (r >> 7) * a.kt * 512 + (r & 31) * 16 + ((r & 127) >> 5) * 4 + g;
+  }
+  const uint16_t* xrow = reinterpret_cast<const uint16_t*>(a.x) + (int64_t)min(r16, a.M - 1) * a.ld_x;
+  const int k0 = kFmt == MXFP4_E4M3 ? 16 * g : 32 * g, k1 = kFmt == MXFP4_E4M3 ? 64 + 16 * g : 32 * g + 16;
+  v4f acc[kB];
+#pragma unroll
+  for (int i = 0; i < kB; ++i) acc[i] = v4f{0.f, 0.f, 0.f, 0.f};
+  for (int t = t0; t < t1; t += kU) {
+    uint4 wv[kU][kB];
+    uint32_t ws[kU][kB], xv[kU][16];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {  // tiles past the wave's range re-read its last one and are not used
+      const int64_t tu = min(t + u, t1 - 1);
+#pragma unroll
+      for (int i = 0; i < kB; ++i) {
+        wv[u][i] = *reinterpret_cast<const uint4*>(wp[i] + tu * 1024);
+        ws[u][i] = sp[i][tu * 512];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const int tu = min(t + u, t1 - 1);
+      load16p<kT>(xrow, tu * 128 + k0, a.K, a.vec_x, xv[u]);
+      load16p<kT>(xrow, tu * 128 + k1, a.K, a.vec_x, xv[u] + 8);
+    }
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      if (t + u >= t1) break;
+      uint32_t xs;
+      const v8i xo = operand<kT, kFmt>(xv[u], g, xs);
+#pragma unroll
+      for (int i = 0; i < kB; ++i) {
+        const v8i wo = {(int)wv[u][i].x, (int)wv[u][i].y, (int)wv[u][i].z, (int)wv[u][i].w, 0, 0, 0, 0};
+        acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wo, xo, acc[i], 4, kFmt == MXFP4_E4M3 ? 0 : 4, 0,
+                                                                  (int)ws[u][i], 0, (int)xs);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kB; ++i) part[wave][i][lane] = f32x4{acc[i][0], acc[i][1], acc[i][2], acc[i][3]};
+  __syncthreads();
+  if (wave) return;
+  float v[kB][4];
+#pragma unroll
+  for (int i = 0; i < kB; ++i) {
+    f32x4 s = part[0][i][lane];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) s += part[w][i][lane];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[i][q] = s[q];
+  }
+  // lane: token r16, weight rows 4 g + 0..3 of the 16, which are 4 consecutive columns (the PI order)
+  const int half = (int)(blk & 1);
+  const int64_t c = (blk >> 1) * 32 + (g & 1) * 16 + (2 * half + (g >> 1)) * 4;
+  if (r16 >= a.M) return;
+  T* out = reinterpret_cast<T*>(a.c) + r16 * a.ldc;
+  if constexpr (kGated) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if (a.add && c + q < a.N) {
+        const T* ad = reinterpret_cast<const T*>(a.add) + r16 * a.ld_add;
+        v[0][q] += Elem<kT>::get(ad[c + q]);
+        v[1][q] += Elem<kT>::get(ad[a.N + c + q]);
+      }
+      v[0][q] = (a.fn == MXFP4_SILU ? gate_fn<MXFP4_SILU>(v[0][q]) : gate_fn<MXFP4_GELU>(v[0][q])) * v[1][q];
+    }
+  }
+  store_run<kT, 4>(out, c, a.N, a.vec_c, v[0]);
+}
+
+template <int kT, int kFmt, bool kGated>
+void launch(const FewArgs& a, unsigned blocks, hipStream_t st) {
+  if (a.kt >= 16) few_kernel<kT, kFmt, kGated, 8><<<blocks, 512, 0, st>>>(a);
+  else few_kernel<kT, kFmt, kGated, 4><<<blocks, 256, 0, st>>>(a);
+}
+
+template <bool kGated>
+int run(FewArgs& a, int64_t fmt, int64_t type, const char* what, hipStream_t st) {
+  const int64_t blocks = ((int64_t)a.N + 31) / 32 * 2;
+  a.kt = (a.K + 127) / 128;
+  a.vec_x = mx_aligned(a.x, 16) && a.ld_x % 8 == 0;
+  a.vec_c = mx_aligned(a.c, 8) && a.ldc % 4 == 0;
+  const bool f8 = fmt == MXFP4_E4M3;
+  if (type == MXFP4_BF16)
+    f8 ? launch<MXFP4_BF16, MXFP4_E4M3, kGated>(a, (unsigned)blocks, st) : launch<MXFP4_BF16, MXFP4_E2M1, kGated>(a, (unsigned)blocks, st);
+  else
+    f8 ? launch<MXFP4_F16, MXFP4_E4M3, kGated>(a, (unsigned)blocks, st) : launch<MXFP4_F16, MXFP4_E2M1, kGated>(a, (unsigned)blocks, st);
+  MX_CHECK_LAUNCH(what);
+  return MXFP8_OK;
+}
+
+int check(const char* what, const void* x, int64_t ld_x, int64_t fmt, const void* b, const void* sb, int64_t M, int64_t N,
+          int64_t K, const void* c, int64_t ldc, int64_t type) {
+  MX_CHECK_ARG(M >= 0 && M <= MXFP4_FEW_ROWS && N > 0 && N < (1LL << 29) && K > 0 && K < (1LL << 26),
+               "%s: bad shape (M=%lld N=%lld K=%lld; at most %d rows)", what, (long long)M, (long long)N, (long long)K,
+               MXFP4_FEW_ROWS);
+  MX_CHECK_ARG(fmt == MXFP4_E2M1 || fmt == MXFP4_E4M3, "%s: unknown format %lld", what, (long long)fmt);
+  MX_CHECK_ARG(type == MXFP4_BF16 || type == MXFP4_F16, "%s: bf16 or f16 (type %lld)", what, (long long)type);
+  if (M == 0) return MXFP8_OK;
+  MX_CHECK_ARG(x && b && sb && c && ld_x >= 0 && ldc >= N, "%s: null pointer or bad stride", what);
+  MX_CHECK_ARG(mx_aligned(x, 2) && mx_aligned(b, 16) && mx_aligned(sb, 16) && mx_aligned(c, 2), "%s: misaligned buffer",
+               what);
+  return MXFP8_OK;
+}
+
+}  // namespace
+
+extern "C" int mxfp4_few(const void* x, int64_t ld_x, int64_t fmt, const void* b, const void* sb, int64_t M, int64_t N,
+                         int64_t K, void* c, int64_t ldc, int64_t type, void* stream) {
+  if (int rc = check("mxfp4_few", x, ld_x, fmt, b, sb, M, N, K, c, ldc, type)) return rc;
+  if (M == 0) return MXFP8_OK;
+  FewArgs a{x, ld_x, (const uint8_t*)b, (const uint8_t*)sb, (int)M, (int)N, (int)K, 0, c, ldc, nullptr, 0, 0, 0, 0};
+  return run<false>(a, fmt, type, "mxfp4_few", (hipStream_t)stream);
+}
+
+extern "C" int mxfp4_few_gated(const void* x, int64_t ld_x, int64_t fmt, const void* b, const void* sb, int64_t M,
+                               int64_t N, int64_t K, const void* add, int64_t ld_add, int64_t fn, void* h, int64_t ldh,
+                               int64_t type, void* stream) {
+  if (int rc = check("mxfp4_few_gated", x, ld_x, fmt, b, sb, M, N, K, h, ldh, type)) return rc;
+  MX_CHECK_ARG(fn == MXFP4_SILU || fn == MXFP4_GELU, "mxfp4_few_gated: unknown gate function %lld", (long long)fn);
+  MX_CHECK_ARG(!add || ((ld_add == 0 || ld_add >= 2 * N) && mx_aligned(add, 2)), "mxfp4_few_gated: bad addend");
+  if (M == 0) return MXFP8_OK;
+  FewArgs a{x, ld_x, (const uint8_t*)b, (const uint8_t*)sb, (int)M, (int)N, (int)K, 0, h, ldh, add, ld_add, (int)fn, 0, 0};
+  return run<true>(a, fmt, type, "mxfp4_few_gated", (hipStream_t)stream);
+}

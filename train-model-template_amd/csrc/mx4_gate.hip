@@ -1,0 +1,128 @@
+// Backward of the gated block's gate: from the saved [g | u] and dh, du = dh fn(g) and dg = dh u fn'(g), quantized straight
+// from fp32 into the operand of the product with [W_gate; W_up] (and, where an addend wants its gradient, rounded to the
+// activations' type).
+//
+// What bounds it: memory, 6 bytes read and 2 (E4M3) or 1 (E2M1) written for each column of a row.  The saved values lie in
+// the order of the forward epilogue's lanes, which is this kernel's order too: lane l of a wave holds row l % 32 and 16
+// columns of a 32 x 32 block, a 32-column scale block is two lanes, and every load of the saved values is 1 KB in a row.
+#include "abi_common.h"
+#include "mx4_device.h"
+
+using namespace mx4;
+
+namespace {
+
+constexpr int kThreads = 256;
+
+struct BwdArgs {
+  const void* gu;
+  const void* dh;
+  int64_t ld_dh;
+  int M, N;
+  uint8_t* q;
+  uint8_t* s;
+  void* dgu;
+  int vec_dh, vec_dgu;
+};
+
+// 16 codes of v (its other 16 in lane l ^ 32) at row m, column c of an operand with ct column tiles; scale 0 past the rows
+template <int kFmt>
+__device__ __forceinline__ void quant_store(const float* v, int64_t m, int64_t c, int64_t ct, bool live, uint8_t* q,
+                                            uint8_t* s, int lane) {
+  uint32_t a, b;
+  pair32(max(absmax8(v), absmax8(v + 8)), a, b);
+  const uint32_t e = block_exponent<kFmt>(max(a, b));
+  uint32_t c0[2], c1[2];
+  encode8<kFmt>(v, e, c0);
+  encode8<kFmt>(v + 8, e, c1);
+  if (live) {
+    uint8_t* p = q + code_offset<kFmt>(m, c, ct);
+    if constexpr (kFmt == MXFP4_E4M3) *reinterpret_cast<uint4*>(p) = make_uint4(c0[0], c0[1], c1[0], c1[1]);
+    else *reinterpret_cast<uint2*>(p) = make_uint2(c0[0], c1[0]);
+  }
+  if (lane < 32) s[blocked_offset(m, c >> 5, ct)] = live ? (uint8_t)e : (uint8_t)0;
+}
+
+template <int kT, int kFn, int kFmt>
+__global__ __launch_bounds__(kThreads) void gate_bwd_kernel(const BwdArgs a) {
+  typedef typename Elem<kT>::T T;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, hi = lane >> 5;
+  const int64_t nblk = (a.N + 31) / 32, tiles = (a.N + 127) / 128;
+  const int64_t m = (int64_t)blockIdx.y * 128 + w * 32 + (lane & 31);  // scale bytes of a tile's 128 rows are all written
+  const int64_t mc = min(m, (int64_t)a.M - 1);
+  const bool live = m < a.M;
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {
+    const int64_t cb = (int64_t)blockIdx.x * 128 + b * 32, c = cb + hi * 16;
+    float dg[16], du[16];
+    if (cb < a.N) {
+      float g[16], u[16], d[16];
+      const T* s = reinterpret_cast<const T*>(a.gu) + saved_offset(mc, c, nblk);
+      load8<kT>(s, g);
+      load8<kT>(s + 512, g + 8);
+      load8<kT>(s + 1024, u);
+      load8<kT>(s + 1536, u + 8);
+      const T* p = reinterpret_cast<const T*>(a.dh) + mc * a.ld_dh;
+      if (a.vec_dh && cb + 32 <= a.N) {
+        load8<kT>(p + c, d);
+        load8<kT>(p + c + 8, d + 8);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const T t = p[min(c + i, (int64_t)a.N - 1)];
+          d[i] = Elem<kT>::get(t);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float df;
+        const float f = gate_fn<kFn>(g[i], df);
+        // the saved values past the last column are undefined
+        dg[i] = c + i < a.N ? d[i] * u[i] * df : 0.f;
+        du[i] = c + i < a.N ? d[i] * f : 0.f;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) dg[i] = du[i] = 0.f;
+    }
+    quant_store<kFmt>(dg, m, c, 2 * tiles, live, a.q, a.s, lane);
+    quant_store<kFmt>(du, m, tiles * 128 + c, 2 * tiles, live, a.q, a.s, lane);
+    if (a.dgu && live) {
+      T* o = reinterpret_cast<T*>(a.dgu) + m * 2 * a.N;
+      store_run<kT, 16>(o, c, a.N, a.vec_dgu, dg);
+      store_run<kT, 16>(o + a.N, c, a.N, a.vec_dgu, du);
+    }
+  }
+}
+
+template <int kT, int kFn>
+void launch(const BwdArgs& a, int64_t fmt, dim3 grid, hipStream_t st) {
+  if (fmt == MXFP4_E4M3) gate_bwd_kernel<kT, kFn, MXFP4_E4M3><<<grid, kThreads, 0, st>>>(a);
+  else gate_bwd_kernel<kT, kFn, MXFP4_E2M1><<<grid, kThreads, 0, st>>>(a);
+}
+
+}  // namespace
+
+extern "C" int mxfp4_gated_bwd(const void* gu, const void* dh, int64_t ld_dh, int64_t M, int64_t N, int64_t fn,
+                               int64_t type, int64_t fmt, void* q, void* s, void* dgu, void* stream) {
+  MX_CHECK_ARG(M >= 0 && N > 0 && M < (1LL << 30) && N < (1LL << 29), "mxfp4_gated_bwd: bad shape (M=%lld N=%lld)",
+               (long long)M, (long long)N);
+  MX_CHECK_ARG(type == MXFP4_BF16 || type == MXFP4_F16, "mxfp4_gated_bwd: bf16 or f16 (type %lld)", (long long)type);
+  MX_CHECK_ARG(fn == MXFP4_SILU || fn == MXFP4_GELU, "mxfp4_gated_bwd: unknown gate function %lld", (long long)fn);
+  MX_CHECK_ARG(fmt == MXFP4_E2M1 || fmt == MXFP4_E4M3, "mxfp4_gated_bwd: unknown format %lld", (long long)fmt);
+  if (M == 0) return MXFP8_OK;
+  MX_CHECK_ARG(gu && dh && q && s && ld_dh >= N, "mxfp4_gated_bwd: null pointer or bad stride");
+  MX_CHECK_ARG(mx_aligned(gu, 16) && mx_aligned(dh, 2) && mx_aligned(q, 16) && mx_aligned(s, 16) && mx_aligned(dgu, 2),
+               "mxfp4_gated_bwd: misaligned buffer");
+  MX_CHECK_ARG((M + 127) / 128 <= 65535, "mxfp4_gated_bwd: too many rows");
+  const BwdArgs a{gu, dh, ld_dh, (int)M, (int)N, (uint8_t*)q, (uint8_t*)s, dgu, mx_aligned(dh, 16) && ld_dh % 8 == 0,
+                  mx_aligned(dgu, 16) && N % 8 == 0};
+  const dim3 grid((unsigned)((N + 127) / 128), (unsigned)((M + 127) / 128));
+  const hipStream_t st = (hipStream_t)stream;
+  if (type == MXFP4_BF16)
+    fn == MXFP4_SILU ? launch<MXFP4_BF16, MXFP4_SILU>(a, fmt, grid, st) : launch<MXFP4_BF16, MXFP4_GELU>(a, fmt, grid, st);
+  else
+    fn == MXFP4_SILU ? launch<MXFP4_F16, MXFP4_SILU>(a, fmt, grid, st) : launch<MXFP4_F16, MXFP4_GELU>(a, fmt, grid, st);
+  MX_CHECK_LAUNCH("mxfp4_gated_bwd");
+  return MXFP8_OK;
+}
