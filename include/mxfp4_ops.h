@@ -94,13 +94,13 @@ int mxfp4_few_gated(const void* x, int64_t ld_x, int64_t fmt, const void* b, con
  * loss [T] fp32 or null; grad [T, V] of the logits' type (row stride ld_grad; may be the logits themselves) or null, with
  * weight [T] fp32 (null: 1).  Rows without a teacher entry of positive mass, and the gradient of rows of weight 0, are 0
  * whatever the logits hold.
- * parts: pieces a row is split into.  1: one launch, ws unused.  More: two launches that pass distill_workspace_size bytes
+ * parts: pieces a row is split into, of at most 2^18 columns (distill_parts).  1: one launch, ws unused.  More: two launches that pass distill_workspace_size bytes
  * in ws.  stages: 3 both; 1 only the statistics into ws; 2 only the loss and gradient from them (parts > 1, or ws kept). */
 #define DISTILL_STATS 1
 #define DISTILL_FINISH 2
 #define DISTILL_MAX_K 1024
 #define DISTILL_MAX_PARTS 256
-int64_t distill_parts(int64_t T, int64_t V, int64_t rest);
+int64_t distill_parts(int64_t T, int64_t V);
 int64_t distill_workspace_size(int64_t T, int64_t k, int64_t parts);
 int distill_topk_kl(const void* logits, int64_t type, int64_t ld, int64_t T, int64_t V, const void* idx, int64_t idx_bytes,
                     int64_t ld_idx, const float* t, int64_t ld_t, int64_t k, float tau, const float* lse,

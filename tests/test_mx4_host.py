@@ -105,18 +105,18 @@ def test_refusals(lib):
     _refused(lib, kl(stages=4), "plan")
     _refused(lib, kl(grad=P, ldg=99), "stride")
     _refused(lib, kl(type=5), "element type")
-    _refused(lib, kl(V=1 << 20, lse=P), "too few parts")
+    _refused(lib, kl(V=1 << 20), "too few parts")
 
 
 def test_plans(lib):
     assert lib.mxfp4_gated_saved_elems(I(33), I(65)) == 2 * 3 * 2048
-    parts = lambda T, V, rest: lib.distill_parts(I(T), I(V), I(rest))  # noqa: E731
-    assert parts(4096, 65536, 0) == 1 and parts(1, 1000, 0) == 1 and parts(1, 65536, 0) > 1
+    parts = lambda T, V: lib.distill_parts(I(T), I(V))  # noqa: E731
+    assert parts(4096, 65536) == 1 and parts(1, 1000) == 1 and parts(1, 65536) > 1
     for T in (1, 7, 300, 5000):
         for V in (1, 1000, 248001, 1 << 22):
-            p = parts(T, V, 1)
+            p = parts(T, V)
             assert 1 <= p <= 256 and -(-V // p) <= 1 << 18
-    assert lib.distill_workspace_size(I(3), I(5), I(2)) == 3 * 2 * 8 + 3 * 5 * 4
+    assert lib.distill_workspace_size(I(3), I(5), I(2)) == 3 * 2 * 8 + 3 * 5 * 8
 
 
 def test_cpu_tensors_and_names_are_refused():

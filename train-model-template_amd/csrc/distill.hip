@@ -4,12 +4,13 @@
 //   loss = tau^2 (sum_S p (log p - log q) + p_r (log p_r - log q_r)),   q_r = sum of q outside S
 //   d loss / d z_j = tau (q_j P - p_j) on S, P = sum p + p_r;  tau q_j (P - p_r / q_r) elsewhere
 // Without the rest bucket p_r = 0.  One pass over the row keeps a running maximum m and the sum s of exp((z - m) / tau) in
-// fp32; with the bucket it leaves out S (a bit for every column in LDS), so that q_r comes from its own maximum and sum and
-// not from a difference.  The factors exp((m - M) / tau) / sum and p_r / s that the gradient needs are at most 1 each.
-// z - m is taken before the division by tau: rows of the type's lowest value stay uniform.
+// fp32 over the columns outside S (a bit for every column in LDS says which), and S is added from its k values: q_r has its
+// own maximum and sum and is no difference.  The factors exp((m - M) / tau) / sum and p_r / s that the gradient needs are at
+// most 1 each.  z - m is taken before the division by tau: rows of the type's lowest value stay uniform.
 //
-// What bounds it: memory, the logits read once and the gradient written once.  A workgroup takes a row (its second reading
-// comes from the cache); few rows are split into pieces over two launches, joined by the second.
+// What bounds it: memory, the logits read once and the gradient written once.  A workgroup takes a row and holds it, or its
+// first 128K (64K in fp32) columns, in registers between the two passes; what is left comes from the cache the second time.
+// Few rows are split into pieces over two launches, joined by the second.
 #include <algorithm>
 
 #include "abi_common.h"
@@ -19,10 +20,9 @@ using namespace mx4;
 
 namespace {
 
-constexpr int kThreads = 512, kWaves = kThreads / 64;
 constexpr float kLowest = -3.4028234663852886e38f;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int64_t kMaxPiece = 1 << 18;  // columns of a piece with the rest bucket: its bits take 32 KB
+constexpr int64_t kMaxPiece = 1 << 18;  // columns of a piece: its bits take 32 KB
 
 struct Args {
   const void* z;
@@ -40,10 +40,11 @@ struct Args {
   void* grad;
   int64_t ld_grad;
   int parts;
-  int wgs;        // workgroups of a row in this launch: parts, or 1 for the loss alone
-  int64_t piece;  // vectors of a piece
-  float2* stats;  // [T][parts]
-  float* zs;      // [T][k] logits of the entries
+  int wgs;         // workgroups of a row in this launch: parts, or 1 for the loss alone
+  int64_t piece;   // vectors of a piece
+  int bit_words;   // words of LDS for the bits
+  float2* stats;   // [T][parts] running maximum and sum of the piece
+  float2* entries; // [T][k] logit of the entry, and 1 if it is the first of its column
 };
 
 struct Sum {
@@ -53,28 +54,22 @@ __device__ __forceinline__ Sum join(Sum a, Sum b, float c) {
   const float m = fmaxf(a.m, b.m);
   return Sum{m, a.s * __builtin_amdgcn_exp2f((a.m - m) * c) + b.s * __builtin_amdgcn_exp2f((b.m - m) * c)};
 }
-
 template <class F>
 __device__ __forceinline__ float wave_reduce(float v, F f) {
 #pragma unroll
   for (int o = 32; o; o >>= 1) v = f(v, __shfl_xor(v, o));
   return v;
 }
-template <class F>
-__device__ __forceinline__ float block_reduce(float v, F f, float* sh) {
-  v = wave_reduce(v, f);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
-  __syncthreads();
-  float r = sh[0];
-#pragma unroll
-  for (int w = 1; w < kWaves; ++w) r = f(r, sh[w]);
-  return r;
+__device__ __forceinline__ float wave_sum(float v) {
+  return wave_reduce(v, [](float a, float b) { return a + b; });
 }
+__device__ __forceinline__ float wave_max(float v) {  // NaN stays
+  return wave_reduce(v, [](float a, float b) { return (a > b || a != a) ? a : b; });
+}
+template <int kWaves>
 __device__ __forceinline__ Sum block_join(Sum a, float c, float* sh) {
 #pragma unroll
   for (int o = 32; o; o >>= 1) a = join(a, Sum{__shfl_xor(a.m, o), __shfl_xor(a.s, o)}, c);
-  __syncthreads();
   if ((threadIdx.x & 63) == 0) {
     sh[threadIdx.x >> 6] = a.m;
     sh[kWaves + (threadIdx.x >> 6)] = a.s;
@@ -85,58 +80,68 @@ __device__ __forceinline__ Sum block_join(Sum a, float c, float* sh) {
   for (int w = 1; w < kWaves; ++w) r = join(r, Sum{sh[w], sh[kWaves + w]}, c);
   return r;
 }
-__device__ __forceinline__ float fadd(float a, float b) { return a + b; }
-__device__ __forceinline__ float fmax2(float a, float b) { return fmaxf(a, b); }
 
 template <int kT>
 struct Vec {
   static constexpr int n = kT == MXFP4_F32 ? 4 : 8;  // elements of 16 bytes
 };
 template <int kT>
-__device__ __forceinline__ void load_vec(const typename Elem<kT>::T* p, float* v) {
-  if constexpr (kT == MXFP4_F32) {
-    const f32x4 a = *reinterpret_cast<const f32x4*>(p);
+__device__ __forceinline__ void unpack_vec(uint4 u, float* v) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = a[i];
-  } else {
-    load8<kT>(p, v);
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (kT == MXFP4_F32) {
+      v[i] = __uint_as_float(w[i]);
+    } else if constexpr (kT == MXFP4_BF16) {
+      v[2 * i] = bf16_lo(w[i]);
+      v[2 * i + 1] = bf16_hi(w[i]);
+    } else {
+      const f16x2 h = __builtin_bit_cast(f16x2, w[i]);
+      v[2 * i] = (float)h[0];
+      v[2 * i + 1] = (float)h[1];
+    }
   }
 }
 
-// kStats: the running maximum and sum of this workgroup's piece.  kFinish: loss and gradient, from the sums of all pieces.
-// Both: the piece is the whole row and nothing passes through memory.
-template <int kT, bool kRest, bool kStats, bool kFinish>
-__global__ __launch_bounds__(kThreads) void distill_kernel(const Args a) {
+template <int kT>
+__device__ __forceinline__ uint4 pack_vec(float* v) {
+  if constexpr (kT == MXFP4_F32)
+    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+  else
+    return make_uint4(round2<kT>(v[0], v[1]), round2<kT>(v[2], v[3]), round2<kT>(v[4], v[5]), round2<kT>(v[6], v[7]));
+}
+
+// What a row's entries give without the row's sums (one wave computes it while the others read the row)
+struct Teacher {
+  float live;    // a teacher entry of positive mass
+  float psum;    // sum of p
+  float rest;    // p_r
+  float zm, own; // maximum and sum of exp((z - zm) / tau) over S
+  float a;       // sum of p (log p - (z - zm) / tau)
+  float dup;     // a column comes twice
+};
+
+enum Mode { kWhole, kStats, kFinish };  // a whole row; a piece's sums; loss and gradient of a piece from all sums
+
+template <int kT, int kMode, int kThreads, int kHold>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kHold > 8 ? 4 : 8)))
+void distill_kernel(const Args a) {
   typedef typename Elem<kT>::T T;
-  constexpr int n = Vec<kT>::n;
-  extern __shared__ uint32_t bits[];  // a bit for every column of the piece: S
-  __shared__ int s_idx[DISTILL_MAX_K];
-  __shared__ float s_z[DISTILL_MAX_K], s_p[DISTILL_MAX_K];
+  constexpr int n = Vec<kT>::n, kWaves = kThreads / 64;
+  constexpr bool kStream = kHold == 0 || kHold == 16;  // columns past what the registers hold
+  extern __shared__ uint32_t bits[];  // a bit for every column of the piece: S; then the entries
   __shared__ float sh[2 * kWaves];
-  const int tid = threadIdx.x;
+  __shared__ Teacher teacher;
+  int* const s_idx = reinterpret_cast<int*>(bits + a.bit_words);  // column, < 0: padding
+  int* const s_first = s_idx + a.k;
+  float* const s_z = reinterpret_cast<float*>(s_first + a.k);
+  float* const s_p = s_z + a.k;
+  const int tid = threadIdx.x, k = a.k;
   const int64_t row = blockIdx.x / (uint32_t)a.wgs;
   const int part = (int)(blockIdx.x - row * a.wgs);
   const T* z = reinterpret_cast<const T*>(a.z) + row * a.ld;
-  const float c = kLog2e / a.tau;
+  const float c = kLog2e / a.tau, itau = 1.f / a.tau;
   const float weight = a.weight ? a.weight[row] : 1.f;
-
-  // ---- the teacher's entries; s_idx < 0: padding
-  float tmax = kLowest;
-  for (int i = tid; i < a.k; i += kThreads) {
-    const int64_t o = row * a.ld_idx + i;
-    const int64_t j = a.idx8 ? reinterpret_cast<const int64_t*>(a.idx)[o] : (int64_t)reinterpret_cast<const int32_t*>(a.idx)[o];
-    const float t = a.t[row * a.ld_t + i];
-    const bool ok = j >= 0 && j < a.V && !(t == -__builtin_inff());
-    s_idx[i] = ok ? (int)j : -1;
-    s_p[i] = t;
-    if (ok) {
-      tmax = (t > tmax || t != t) ? t : tmax;
-      s_z[i] = kStats ? Elem<kT>::get(z[j]) : a.zs[row * a.k + i];
-    }
-  }
-  float any = 0.f;
-  for (int i = tid; i < a.k; i += kThreads) any = s_idx[i] >= 0 ? 1.f : any;
-  const bool live = block_reduce(any, fmax2, sh) > 0.f;  // block_reduce's barriers publish s_idx, s_z, s_p
 
   // the row's vectors: `head` elements before the first aligned one, this workgroup's vectors [v0, v1), a tail
   const int head = (int)min((int64_t)((16 - ((uintptr_t)z & 15)) & 15) / (int)sizeof(T), a.V);
@@ -144,227 +149,245 @@ __global__ __launch_bounds__(kThreads) void distill_kernel(const Args a) {
   const int64_t v0 = min((int64_t)part * a.piece, nv), v1 = min(v0 + a.piece, nv);
   const bool first = part == 0, last = part == a.parts - 1;
   const int64_t tail0 = head + nv * n;
-  // columns of this workgroup: [c0, c1)
-  const int64_t c0 = first ? 0 : head + v0 * n, c1 = last ? a.V : head + v1 * n;
+  const int64_t c0 = first ? 0 : head + v0 * n, c1 = last ? a.V : head + v1 * n;  // this workgroup's columns
+  // the piece's vectors by a 32-bit index from a wave-uniform address
+  const char* const zp = reinterpret_cast<const char*>(z + head + v0 * n);
+  const int pv = (int)(v1 - v0);
+  auto load = [&](int v) { return *reinterpret_cast<const uint4*>(zp + (uint32_t)v * 16u); };
 
-  Sum tot{kLowest, 0.f};
-  if constexpr (kStats) {
-    if (live) {
-      // bit b of the piece: column head + v0 n - 8 + b, so that a vector's bits lie in one byte
-      const int64_t b0 = head + v0 * n - 8;
-      if constexpr (kRest) {
-        const int words = (int)((c1 - b0 + 31) >> 5);
-        for (int i = tid; i < words; i += kThreads) bits[i] = 0;
-        __syncthreads();
-        for (int i = tid; i < a.k; i += kThreads)
-          if (s_idx[i] >= c0 && s_idx[i] < c1) atomicOr(&bits[(s_idx[i] - b0) >> 5], 1u << ((s_idx[i] - b0) & 31));
-        __syncthreads();
-      }
-      auto take = [&](float v) {
-        const float m = fmaxf(tot.m, v);
-        tot.s = tot.s * __builtin_amdgcn_exp2f((tot.m - m) * c) + __builtin_amdgcn_exp2f((v - m) * c);
-        tot.m = m;
-      };
-      auto scalar = [&](int64_t j) {
-        if constexpr (kRest) {
-          if (bits[(j - b0) >> 5] >> ((j - b0) & 31) & 1) return;
-        }
-        take(Elem<kT>::get(z[j]));
-      };
-      if (first && tid < head) scalar(tid);
-      if (last && tail0 + tid < a.V) scalar(tail0 + tid);
-      auto vector = [&](int64_t v, float* x) {
-        if constexpr (kRest) {
-          const int64_t b = (v - v0) * n + 8;
-          const uint32_t mask = (bits[b >> 5] >> (b & 31)) & ((1u << n) - 1);
-          if (mask) {
+  uint4 held[kHold > 0 ? kHold : 1];
+  if constexpr (kHold > 0) {
 #pragma unroll
-            for (int i = 0; i < n; ++i) x[i] = (mask >> i & 1) ? -__builtin_inff() : x[i];
-          }
-        }
-        float m = tot.m;
-#pragma unroll
-        for (int i = 0; i < n; ++i) m = fmaxf(m, x[i]);
-        float s = tot.s * __builtin_amdgcn_exp2f((tot.m - m) * c);
-#pragma unroll
-        for (int i = 0; i < n; ++i) s += __builtin_amdgcn_exp2f((x[i] - m) * c);
-        tot = Sum{m, s};
-      };
-      int64_t v = v0 + tid;
-      for (; v + 3 * kThreads < v1; v += 4 * kThreads) {
-        float x[4][n];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) load_vec<kT>(z + head + (v + u * kThreads) * n, x[u]);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) vector(v + u * kThreads, x[u]);
-      }
-      for (; v < v1; v += kThreads) {
-        float x[n];
-        load_vec<kT>(z + head + v * n, x);
-        vector(v, x);
-      }
-      tot = block_join(tot, c, sh);
-    }
-    if constexpr (!kFinish) {
-      if (tid == 0) a.stats[row * a.parts + part] = make_float2(tot.m, tot.s);
-      if (first)
-        for (int i = tid; i < a.k; i += kThreads)
-          if (s_idx[i] >= 0) a.zs[row * a.k + i] = s_z[i];
-      return;
+    for (int u = 0; u < kHold; ++u)
+      if (pv > 0) held[u] = load(min(tid + u * kThreads, pv - 1));
+  }
+
+  // ---- the teacher's entries
+  if constexpr (kMode != kFinish)
+    for (int i = tid; i < a.bit_words; i += kThreads) bits[i] = 0;
+  for (int i = tid; i < k; i += kThreads) {
+    const int64_t o = row * a.ld_idx + i;
+    const int64_t j = a.idx8 ? reinterpret_cast<const int64_t*>(a.idx)[o] : (int64_t)reinterpret_cast<const int32_t*>(a.idx)[o];
+    const float t = a.t[row * a.ld_t + i];
+    const bool ok = j >= 0 && j < a.V && !(t == -__builtin_inff());
+    s_idx[i] = ok ? (int)j : -1;
+    s_p[i] = t;
+    if constexpr (kMode == kFinish) {
+      const float2 e = ok ? a.entries[row * k + i] : make_float2(0.f, 0.f);
+      s_z[i] = e.x;
+      s_first[i] = e.y != 0.f;
     }
   }
-  if constexpr (kFinish) {
-    const bool zero_grad = !live || weight == 0.f;
-    float f = 0.f, big = 0.f, P = 1.f, log_sum = 0.f, scale = 0.f;
-    if (live) {
-      if constexpr (!kStats) {
-        for (int i = tid; i < a.parts; i += kThreads) {
-          const float2 st = a.stats[row * a.parts + i];
-          tot = join(tot, Sum{st.x, st.y}, c);
-        }
-        tot = block_join(tot, c, sh);
+  __syncthreads();
+  const int64_t b0 = head + v0 * n - 8;  // column of bit 0, so that a vector's bits lie in one byte
+  if constexpr (kMode != kFinish) {
+    for (int i = tid; i < k; i += kThreads) {
+      const int j = s_idx[i];
+      s_first[i] = 0;
+      if (j < c0 || j >= c1) continue;
+      const uint32_t bit = 1u << ((j - b0) & 31);
+      s_first[i] = !(atomicOr(&bits[(j - b0) >> 5], bit) & bit);  // one entry of a column is its first
+      s_z[i] = Elem<kT>::get(z[j]);
+      if constexpr (kMode == kStats) a.entries[row * k + i] = make_float2(s_z[i], (float)s_first[i]);
+    }
+    __syncthreads();
+  }
+  if (kMode != kStats && tid < 64) {
+    float tmax = kLowest, zm = kLowest, any = 0.f, dup = 0.f;
+    for (int i = tid; i < k; i += 64)
+      if (s_idx[i] >= 0) {
+        const float t = s_p[i];
+        any = 1.f;
+        tmax = (t > tmax || t != t) ? t : tmax;
+        zm = fmaxf(zm, s_z[i]);
+        dup = s_first[i] ? dup : 1.f;
       }
-      // masses of the teacher; entries that repeat an earlier one's column count once in q
-      tmax = block_reduce(tmax, [](float x, float y) { return (x > y || x != x) ? x : y; }, sh);
-      const float lse = a.lse ? a.lse[row] : 0.f, itau = 1.f / a.tau;
-      float psum = 0.f;
-      for (int i = tid; i < a.k; i += kThreads)
-        if (s_idx[i] >= 0)
-          psum += kRest ? expf(s_p[i] * itau - lse) : __builtin_amdgcn_exp2f((s_p[i] - tmax) * c);
-      psum = block_reduce(psum, fadd, sh);
-      // a rest that is the rounding of the sum is not held against a student with nothing outside S
-      float p_rest = kRest ? fmaxf(1.f - psum, 0.f) : 0.f;
-      if (kRest && tot.s == 0.f && p_rest < 0x1p-16f) p_rest = 0.f;
-      P = kRest ? psum + p_rest : 1.f;
-      big = tot.m;
-      float total = tot.s;
-      if constexpr (kRest) {
-        float zm = kLowest;
-        for (int i = tid; i < a.k; i += kThreads)
-          if (s_idx[i] >= 0) zm = fmaxf(zm, s_z[i]);
-        big = fmaxf(big, block_reduce(zm, fmax2, sh));
-        float own = 0.f;
-        for (int i = tid; i < a.k; i += kThreads) {
-          if (s_idx[i] < 0) continue;
-          bool again = false;
-          for (int o = 0; o < i; ++o) again |= s_idx[o] == s_idx[i];
-          if (!again) own += __builtin_amdgcn_exp2f((s_z[i] - big) * c);
-        }
-        own = block_reduce(own, fadd, sh);
-        total = own + tot.s * __builtin_amdgcn_exp2f((tot.m - big) * c);
+    any = wave_max(any);
+    tmax = wave_max(tmax);
+    zm = wave_max(zm);
+    dup = wave_max(dup);
+    const float lse = a.lse ? a.lse[row] : 0.f;
+    float psum = 0.f, own = 0.f, A = 0.f;
+    for (int i = tid; i < k; i += 64)
+      if (s_idx[i] >= 0) {
+        psum += a.lse ? expf(s_p[i] * itau - lse) : expf((s_p[i] - tmax) * itau);
+        if (s_first[i]) own += __builtin_amdgcn_exp2f((s_z[i] - zm) * c);
       }
-      log_sum = total == 0.f ? 0.f : logf(total);
-      // loss
-      float part_loss = 0.f;
-      for (int i = tid; i < a.k; i += kThreads) {
-        if (s_idx[i] < 0) continue;
-        const float logp = kRest ? s_p[i] * itau - lse : (s_p[i] - tmax) * itau - logf(psum);
-        const float logq = total == 0.f ? -__builtin_inff() : (s_z[i] - big) * itau - log_sum;
+    psum = wave_sum(psum);
+    own = wave_sum(own);
+    const float norm = a.lse ? 0.f : logf(psum);
+    for (int i = tid; i < k; i += 64)
+      if (s_idx[i] >= 0) {
+        const float logp = a.lse ? s_p[i] * itau - lse : (s_p[i] - tmax) * itau - norm;
         const float p = expf(logp);
-        if (p > 0.f || p != p) part_loss += p * (logp - logq);
+        s_p[i] = p;
+        if (p > 0.f || p != p) A += p * (logp - (s_z[i] - zm) * itau);
       }
-      part_loss = block_reduce(part_loss, fadd, sh);
-      if (kRest && p_rest > 0.f)
-        part_loss += p_rest * (logf(p_rest) - ((tot.m - big) * itau + logf(tot.s) - log_sum));
-      if (a.loss && first && tid == 0) a.loss[row] = part_loss * a.tau * a.tau;
-      // gradient outside S: exp((z - m) / tau) f
-      scale = weight * a.tau;
-      if (tot.s != 0.f) {
-        f = P * __builtin_amdgcn_exp2f((tot.m - big) * c) / total;
-        if (kRest) f -= p_rest / tot.s;
-        f *= scale;
-      }
-      if (a.grad) {
-        // s_p becomes the gradient on S, s_idx < 0 for the columns of other pieces and repeated entries
-        __syncthreads();
-        float gs[(DISTILL_MAX_K + kThreads - 1) / kThreads];
-        int keep[(DISTILL_MAX_K + kThreads - 1) / kThreads];
+    A = wave_sum(A);
+    if (tid == 0) teacher = Teacher{any, a.lse ? psum : 1.f, a.lse ? fmaxf(1.f - psum, 0.f) : 0.f, zm, own, A, dup};
+  }
+
+  // ---- the running maximum and sum outside S
+  Sum tot{kLowest, 0.f};
+  if constexpr (kMode != kFinish) {
+    auto scalar = [&](int64_t j) {
+      if (bits[(j - b0) >> 5] >> ((j - b0) & 31) & 1) return;
+      tot = join(tot, Sum{Elem<kT>::get(z[j]), 1.f}, c);
+    };
+    auto vector = [&](int v, uint4 raw) {
+      float x[n];
+      unpack_vec<kT>(raw, x);
+      const int b = v * n + 8;
+      const uint32_t mask = (bits[b >> 5] >> (b & 31)) & ((1u << n) - 1);
+      if (mask) {
 #pragma unroll
-        for (int r = 0; r < (DISTILL_MAX_K + kThreads - 1) / kThreads; ++r) {
-          const int i = tid + r * kThreads;
-          keep[r] = 0;
-          if (i >= a.k || s_idx[i] < 0) continue;
-          float p = 0.f;
-          bool again = false;
-          for (int o = 0; o < a.k; ++o)
-            if (s_idx[o] == s_idx[i]) {
-              again |= o < i;
-              p += expf(kRest ? s_p[o] * itau - lse : (s_p[o] - tmax) * itau - logf(psum));
-            }
-          const float q = total == 0.f ? 0.f : __builtin_amdgcn_exp2f((s_z[i] - big) * c) / total;
-          gs[r] = total == 0.f ? 0.f : (q * P - p) * scale;
-          keep[r] = !again && s_idx[i] >= c0 && s_idx[i] < c1;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int r = 0; r < (DISTILL_MAX_K + kThreads - 1) / kThreads; ++r) {
-          const int i = tid + r * kThreads;
-          if (i >= a.k) continue;
-          if (!keep[r]) s_idx[i] = -1;
-          s_p[i] = gs[r];
-        }
+        for (int i = 0; i < n; ++i) x[i] = (mask >> i & 1) ? -__builtin_inff() : x[i];
       }
-    } else if (a.loss && first && tid == 0) {
-      a.loss[row] = 0.f;
+      float m = tot.m;
+#pragma unroll
+      for (int i = 0; i < n; ++i) m = fmaxf(m, x[i]);
+      float s = tot.s * __builtin_amdgcn_exp2f((tot.m - m) * c);
+#pragma unroll
+      for (int i = 0; i < n; ++i) s += __builtin_amdgcn_exp2f((x[i] - m) * c);
+      tot = Sum{m, s};
+    };
+    if (first && tid < head) scalar(tid);
+    if (last && tail0 + tid < a.V) scalar(tail0 + tid);
+    if constexpr (kHold > 0) {
+#pragma unroll
+      for (int u = 0; u < kHold; ++u) {
+        if (tid + u * kThreads < pv) vector(tid + u * kThreads, held[u]);
+        // one vector unpacked at a time, and none of it kept for the second pass in place of the packed form
+        asm("" : "+v"(held[u].x), "+v"(held[u].y), "+v"(held[u].z), "+v"(held[u].w));
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    if constexpr (kStream) {
+    int v = tid + kHold * kThreads;
+    for (; v + 3 * kThreads < pv; v += 4 * kThreads) {
+      uint4 x[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) x[u] = load(v + u * kThreads);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) vector(v + u * kThreads, x[u]);
+    }
+    for (; v < pv; v += kThreads) vector(v, load(v));
+    }
+  } else {
+    for (int i = tid; i < a.parts; i += kThreads) {
+      const float2 st = a.stats[row * a.parts + i];
+      tot = join(tot, Sum{st.x, st.y}, c);
+    }
+  }
+  tot = block_join<kWaves>(tot, c, sh);
+  if constexpr (kMode == kStats) {
+    if (tid == 0) a.stats[row * a.parts + part] = make_float2(tot.m, tot.s);
+    return;
+  }
+
+  // ---- loss and gradient
+  if constexpr (kMode != kStats) {
+    const Teacher tc = teacher;
+    const bool live = tc.live > 0.f;
+    const float big = fmaxf(tot.m, tc.zm);
+    const float e_rest = __builtin_amdgcn_exp2f((tot.m - big) * c);
+    const float total = tot.s * e_rest + tc.own * __builtin_amdgcn_exp2f((tc.zm - big) * c);
+    // a rest that is the rounding of the sum is not held against a student with nothing outside S
+    const float rest = tot.s == 0.f && tc.rest < 0x1p-16f ? 0.f : tc.rest;
+    if (a.loss && first && tid == 0) {
+      const float log_total = total == 0.f ? 0.f : logf(total);
+      float l = tc.a + tc.psum * ((big - tc.zm) * itau + log_total);
+      if (rest > 0.f) l += rest * (logf(rest) - ((tot.m - big) * itau + logf(tot.s) - log_total));
+      a.loss[row] = live ? l * a.tau * a.tau : 0.f;
     }
     if (!a.grad) return;
+    const bool zero = !live || weight == 0.f || total == 0.f;
+    const float P = a.lse ? tc.psum + rest : 1.f, scale = weight * a.tau;
+    float f = 0.f;  // outside S: exp((z - m) / tau) f
+    if (tot.s != 0.f) f = (P * e_rest / total - (rest > 0.f ? rest / tot.s : 0.f)) * scale;
     T* g = reinterpret_cast<T*>(a.grad) + row * a.ld_grad;
     const bool vec = (((uintptr_t)g ^ (uintptr_t)z) & 15) == 0;
-    auto value = [&](float v) { return zero_grad ? 0.f : __builtin_amdgcn_exp2f((v - tot.m) * c) * f; };
+    auto value = [&](float v) { return zero ? 0.f : __builtin_amdgcn_exp2f((v - tot.m) * c) * f; };
+    if (!vec) {  // the gradient lies otherwise in its 16 bytes than the logits (so it is not in place)
+      for (int64_t j = c0 + tid; j < c1; j += kThreads) g[j] = Elem<kT>::put(value(Elem<kT>::get(z[j])));
+    } else {
     if (first && tid < head) g[tid] = Elem<kT>::put(value(Elem<kT>::get(z[tid])));
     if (last && tail0 + tid < a.V) g[tail0 + tid] = Elem<kT>::put(value(Elem<kT>::get(z[tail0 + tid])));
-    auto out = [&](int64_t v, float* x) {
+    char* const gp = reinterpret_cast<char*>(g + head + v0 * n);
+    auto out = [&](int v, uint4 raw) {
+      float x[n];
+      unpack_vec<kT>(raw, x);
 #pragma unroll
       for (int i = 0; i < n; ++i) x[i] = value(x[i]);
-      store_run<kT, n>(g, head + v * n, a.V, vec, x);
+      *reinterpret_cast<uint4*>(gp + (uint32_t)v * 16u) = pack_vec<kT>(x);
     };
-    int64_t v = v0 + tid;
-    for (; v + 3 * kThreads < v1; v += 4 * kThreads) {
-      float x[4][n];
+    if constexpr (kHold > 0) {
 #pragma unroll
-      for (int u = 0; u < 4; ++u) load_vec<kT>(z + head + (v + u * kThreads) * n, x[u]);
+      for (int u = 0; u < kHold; ++u) {
+        if (tid + u * kThreads < pv) out(tid + u * kThreads, held[u]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    if constexpr (kStream) {
+    int v = tid + kHold * kThreads;
+    for (; v + 3 * kThreads < pv; v += 4 * kThreads) {
+      uint4 x[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) x[u] = load(v + u * kThreads);
 #pragma unroll
       for (int u = 0; u < 4; ++u) out(v + u * kThreads, x[u]);
     }
-    for (; v < v1; v += kThreads) {
-      float x[n];
-      load_vec<kT>(z + head + v * n, x);
-      out(v, x);
+    for (; v < pv; v += kThreads) out(v, load(v));
     }
-    if (zero_grad) return;
+    }
+    if (zero) return;
     __syncthreads();  // this workgroup's stores have completed: S goes over them
-    for (int i = tid; i < a.k; i += kThreads)
-      if (s_idx[i] >= 0) g[s_idx[i]] = Elem<kT>::put(s_p[i]);
+    for (int i = tid; i < k; i += kThreads) {
+      const int j = s_idx[i];
+      if (j < c0 || j >= c1 || !s_first[i]) continue;
+      float p = s_p[i];
+      if (tc.dup != 0.f) {
+        p = 0.f;
+        for (int o = 0; o < k; ++o) p += s_idx[o] == j ? s_p[o] : 0.f;
+      }
+      g[j] = Elem<kT>::put((__builtin_amdgcn_exp2f((s_z[i] - big) * c) / total * P - p) * scale);
+    }
   }
 }
 
-template <int kT, bool kRest>
-void launch(const Args& a, int64_t T, int stages, size_t lds, hipStream_t st) {
-  Args b = a;
-  b.wgs = a.parts;
+template <int kT>
+void launch(const Args& a0, int64_t T, int stages, hipStream_t st) {
+  Args a = a0;
+  a.wgs = a.parts;
   const unsigned grid = (unsigned)(T * a.parts);
+  const size_t entries = (size_t)a.k * 16;
   if (stages == (DISTILL_STATS | DISTILL_FINISH) && a.parts == 1) {
-    distill_kernel<kT, kRest, true, true><<<grid, kThreads, lds, st>>>(b);
+    const size_t lds = a.bit_words * 4 + entries;
+    const int64_t nv = a.V / Vec<kT>::n;
+    if (nv <= 1024) distill_kernel<kT, kWhole, 256, 4><<<grid, 256, lds, st>>>(a);
+    else if (nv <= 4096) distill_kernel<kT, kWhole, 512, 8><<<grid, 512, lds, st>>>(a);
+    else if (nv <= 8192) distill_kernel<kT, kWhole, 1024, 8><<<grid, 1024, lds, st>>>(a);
+    else distill_kernel<kT, kWhole, 1024, 16><<<grid, 1024, lds, st>>>(a);
     return;
   }
-  if (stages & DISTILL_STATS) distill_kernel<kT, kRest, true, false><<<grid, kThreads, lds, st>>>(b);
+  if (stages & DISTILL_STATS) distill_kernel<kT, kStats, 512, 0><<<grid, 512, a.bit_words * 4 + entries, st>>>(a);
   if (stages & DISTILL_FINISH) {
-    b.wgs = a.grad ? a.parts : 1;
-    distill_kernel<kT, kRest, false, true><<<(unsigned)(T * b.wgs), kThreads, 0, st>>>(b);
+    a.wgs = a.grad ? a.parts : 1;
+    a.bit_words = 0;
+    distill_kernel<kT, kFinish, 512, 0><<<(unsigned)(T * a.wgs), 512, entries, st>>>(a);
   }
 }
 
 }  // namespace
 
-extern "C" int64_t distill_parts(int64_t T, int64_t V, int64_t rest) {
+extern "C" int64_t distill_parts(int64_t T, int64_t V) {
   if (T <= 0 || V <= 0) return 1;
-  int64_t parts = std::min((int64_t)1024 / T, V / 8192);
-  if (rest) parts = std::max(parts, (V + kMaxPiece - 1) / kMaxPiece);
+  const int64_t parts = std::max(std::min((int64_t)512 / T, V / 8192), (V + kMaxPiece - 1) / kMaxPiece);
   return std::min<int64_t>(std::max<int64_t>(parts, 1), DISTILL_MAX_PARTS);
 }
 
 extern "C" int64_t distill_workspace_size(int64_t T, int64_t k, int64_t parts) {
-  return T <= 0 || k <= 0 || parts <= 0 ? 0 : T * parts * 8 + T * k * 4;
+  return T <= 0 || k <= 0 || parts <= 0 ? 0 : T * parts * 8 + T * k * 8;
 }
 
 extern "C" int distill_topk_kl(const void* logits, int64_t type, int64_t ld, int64_t T, int64_t V, const void* idx,
@@ -388,19 +411,15 @@ extern "C" int distill_topk_kl(const void* logits, int64_t type, int64_t ld, int
   const int es = type == MXFP4_F32 ? 4 : 2;
   MX_CHECK_ARG(mx_aligned(logits, es) && mx_aligned(grad, es) && mx_aligned(idx, idx_bytes) && mx_aligned(ws, 8),
                "distill_topk_kl: misaligned buffer");
-  const int64_t n = 16 / es, nv = V / n;
-  Args a{logits, ld, V, idx, idx_bytes == 8, ld_idx, t, ld_t, (int)k, tau, lse, weight, loss, grad, ld_grad, (int)parts, 0,
-         std::max<int64_t>((nv + parts - 1) / parts, 1), (float2*)ws, ws ? (float*)((char*)ws + T * parts * 8) : nullptr};
-  const bool rest = lse != nullptr;
-  // a bit for every column of a piece, its head and tail
-  const size_t lds = rest ? ((size_t)(a.piece * n + 8 + 64) / 32 + 2) * 4 : 0;
-  MX_CHECK_ARG(!(rest && (stages & DISTILL_STATS)) || a.piece * n <= kMaxPiece + 8, "distill_topk_kl: too few parts");
+  const int64_t n = 16 / es, nv = V / n, piece = std::max<int64_t>((nv + parts - 1) / parts, 1);
+  MX_CHECK_ARG(piece * n <= kMaxPiece + 8, "distill_topk_kl: too few parts");
+  const Args a{logits, ld, V, idx, idx_bytes == 8, ld_idx, t, ld_t, (int)k, tau, lse, weight, loss, grad, ld_grad, (int)parts,
+               0, piece, (int)((piece * n + 8 + 2 * 8) / 32 + 2),  // a piece's columns, 8 before it, head and tail
+               (float2*)ws, ws ? (float2*)((char*)ws + T * parts * 8) : nullptr};
   const hipStream_t st = (hipStream_t)stream;
-#define RUN(T_) (rest ? launch<T_, true>(a, T, (int)stages, lds, st) : launch<T_, false>(a, T, (int)stages, lds, st))
-  if (type == MXFP4_BF16) RUN(MXFP4_BF16);
-  else if (type == MXFP4_F16) RUN(MXFP4_F16);
-  else RUN(MXFP4_F32);
-#undef RUN
+  if (type == MXFP4_BF16) launch<MXFP4_BF16>(a, T, (int)stages, st);
+  else if (type == MXFP4_F16) launch<MXFP4_F16>(a, T, (int)stages, st);
+  else launch<MXFP4_F32>(a, T, (int)stages, st);
   MX_CHECK_LAUNCH("distill_topk_kl");
   return MXFP8_OK;
 }

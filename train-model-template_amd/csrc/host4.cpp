@@ -1,11 +1,17 @@
 // The host side of the 4-bit operators and of the distillation loss in native code: a call's allocations and launches in
 // one step from Python, as host_path.cpp does for the 8-bit path (a single-token product runs for a few microseconds, which
-// is what the Python around it would cost by itself).  Every function allocates through torch, launches on the stream that
-// it is given through the C-ABI of include/mxfp4_ops.h, does not wait, and runs without the interpreter's lock.  Shapes,
-// types, strides and devices are checked here; an error raises _native.NativeError.
+// is what the Python around it would cost by itself; a training step of a thousand tokens runs for 40, half of what the
+// Python form of its backward nodes took).  Every function allocates through torch, launches on the current stream of the
+// tensors' device through the C-ABI of include/mxfp4_ops.h, does not wait, and runs without the interpreter's lock.
+// Shapes, types, strides and devices are checked here; an error raises _native.NativeError.
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/extension.h>
 
+#include <memory>
 #include <optional>
 #include <stdexcept>
 #include <string>
@@ -38,9 +44,14 @@ int64_t code_bytes(int64_t rows, int64_t cols, int64_t fmt) {
   return pad(rows, 32) * pad(cols, 128) / (fmt == MXFP4_E4M3 ? 1 : 2);
 }
 int64_t scale_bytes(int64_t rows, int64_t cols) { return cdiv(rows, 128) * cdiv(cols, 128) * 512; }
-void* stm(int64_t s) { return reinterpret_cast<void*>(s); }
+// What a call runs under: the tensors' device is current and torch records nothing (the nodes below do it by hand)
+struct Scope {
+  c10::OptionalDeviceGuard device;
+  at::AutoDispatchBelowADInplaceOrView below;
+  void* stream;
+  explicit Scope(const Tensor& t) : device(t.device()), stream(c10::hip::getCurrentHIPStream(t.get_device()).stream()) {}
+};
 void* ptr(const Tensor& t) { return t.data_ptr(); }
-void* ptr(const OptT& t) { return t ? t->data_ptr() : nullptr; }
 
 int64_t type_of(const Tensor& t, const char* what) {
   switch (t.scalar_type()) {
@@ -96,219 +107,394 @@ struct Temp {
   }
 };
 
-std::tuple<Tensor, Tensor> quant(const Tensor& x, int64_t fmt, int64_t order, int64_t stream) {
+// ------------------------------------------------------------------ quantization and products of MX operands
+std::tuple<Tensor, Tensor> quant(const Tensor& x, int64_t fmt, int64_t order) {
   const char* what = "mx4_quant";
   gpu(x, what);
-  c10::OptionalDeviceGuard guard(x.device());
+  const Scope sc(x);
   need(x.dim() == 2, what, "a matrix");
   const Tensor m = rows_of(x);
   Operand o = operand(m.size(0), m.size(1), fmt, m);
   ok(mxfp4_quant(ptr(m), type_of(m, what), m.size(0), m.size(1), ld_of(m), fmt, ptr(o.q), ptr(o.s), order, nullptr, nullptr,
-                 0, 0, 0, stm(stream)),
+                 0, 0, 0, sc.stream),
      "mxfp4_quant");
   return {o.q, o.s};
 }
 
 // both axes from one read, each in its row order
-std::tuple<Tensor, Tensor, Tensor, Tensor> quant_both(const Tensor& x, int64_t fmt, int64_t order, int64_t stream) {
+std::tuple<Tensor, Tensor, Tensor, Tensor> quant_both(const Tensor& x, int64_t fmt, int64_t order) {
   const char* what = "mx4_quant";
   gpu(x, what);
-  c10::OptionalDeviceGuard guard(x.device());
+  const Scope sc(x);
   need(x.dim() == 2, what, "a matrix");
   const Tensor m = rows_of(x);
   const int64_t R = m.size(0), C = m.size(1);
   Operand o = operand(R, C, fmt, m), t = operand(C, R, fmt, m);
   ok(mxfp4_quant(ptr(m), type_of(m, what), R, C, ld_of(m), fmt, ptr(o.q), ptr(o.s), order, ptr(t.q), ptr(t.s), order, 0,
-                 cdiv(R, 128), stm(stream)),
+                 cdiv(R, 128), sc.stream),
      "mxfp4_quant");
   return {o.q, o.s, t.q, t.s};
 }
 
-// gate and up [N, K] -> their common operand along K and [K, 2 pad(N, 128)] along N
-std::tuple<Tensor, Tensor, Tensor, Tensor> quant_gate_up(const Tensor& wg, const Tensor& wu, int64_t stream) {
-  const char* what = "GatedWeight";
-  gpu(wg, what);
-  same(wg, wu, what);
-  need(wg.dim() == 2 && wg.sizes() == wu.sizes() && wg.scalar_type() == wu.scalar_type() && wg.numel() > 0, what,
-       "two matrices of one shape and type");
-  c10::OptionalDeviceGuard guard(wg.device());
-  const int64_t N = wg.size(0), K = wg.size(1), nt = cdiv(N, 128);
-  Operand o = operand(2 * pad(N, 32), K, MXFP4_E2M1, wg), t = operand(K, 2 * nt * 128, MXFP4_E2M1, wg);
-  for (int i = 0; i < 2; ++i) {
-    const Tensor m = rows_of(i ? wu : wg);
-    ok(mxfp4_quant(ptr(m), type_of(m, what), N, K, ld_of(m), MXFP4_E2M1, ptr(o.q), ptr(o.s),
-                   i ? MXFP4_ROWS_UP : MXFP4_ROWS_GATE, ptr(t.q), ptr(t.s), MXFP4_ROWS_PI, i * nt, 2 * nt, stm(stream)),
-       "mxfp4_quant");
-  }
-  return {o.q, o.s, t.q, t.s};
-}
-
-Tensor dequant(const Tensor& q, const Tensor& s, int64_t rows, int64_t cols, int64_t fmt, at::ScalarType dt, int64_t stream) {
+Tensor dequant(const Tensor& q, const Tensor& s, int64_t rows, int64_t cols, int64_t fmt, at::ScalarType dt) {
   const char* what = "mx4_dequant";
   gpu(q, what);
-  c10::OptionalDeviceGuard guard(q.device());
+  same(q, s, what);
+  const Scope sc(q);
   need(q.numel() >= code_bytes(rows, cols, fmt) && s.numel() >= scale_bytes(rows, cols), what, "operand too small");
   Tensor out = empty({rows, cols}, dt, q);
-  ok(mxfp4_dequant(ptr(q), ptr(s), rows, cols, fmt, ptr(out), type_of(out, what), stm(stream)), "mxfp4_dequant");
+  ok(mxfp4_dequant(ptr(q), ptr(s), rows, cols, fmt, ptr(out), type_of(out, what), sc.stream), "mxfp4_dequant");
   return out;
 }
 
 Tensor gemm(const Tensor& q, const Tensor& s, int64_t fmt, const Tensor& bq, const Tensor& bs, int64_t order, int64_t M,
-            int64_t N, int64_t K, at::ScalarType dt, int64_t stream) {
+            int64_t N, int64_t K, at::ScalarType dt) {
   const char* what = "mx4_mm";
   gpu(q, what);
-  same(q, bq, what);
-  c10::OptionalDeviceGuard guard(q.device());
+  for (const Tensor* t : {&s, &bq, &bs}) same(q, *t, what);
+  const Scope sc(q);
   need(q.numel() >= code_bytes(M, K, fmt) && s.numel() >= scale_bytes(M, K) && bq.numel() >= code_bytes(N, K, MXFP4_E2M1) &&
            bs.numel() >= scale_bytes(N, K),
        what, "operand too small");
   Tensor out = empty({M, N}, dt, q);
   if (M && N && !K) return out.zero_();
   if (M && N)
-    ok(mxfp4_gemm(ptr(q), ptr(s), fmt, ptr(bq), ptr(bs), order, M, N, pad(K, 128), ptr(out), N, type_of(out, what),
-                  stm(stream)),
+    ok(mxfp4_gemm(ptr(q), ptr(s), fmt, ptr(bq), ptr(bs), order, M, N, pad(K, 128), ptr(out), N, type_of(out, what), sc.stream),
        "mxfp4_gemm");
   return out;
 }
 
-// x [.., K] with a weight [N, K] in the PI order
-Tensor linear(const Tensor& x, const Tensor& wq, const Tensor& ws, int64_t N, int64_t K, int64_t fmt, int64_t stream) {
+// ------------------------------------------------------------------ the frozen weight of a linear layer
+struct Weight {
+  int64_t N, K;
+  Tensor q, s;    // along K, rows in the PI order
+  Tensor qt, st;  // of the transpose, along N; undefined without it
+};
+using WeightP = std::shared_ptr<Weight>;
+
+WeightP make_weight(const Tensor& w, bool transpose) {
+  gpu(w, "Weight");
+  if (w.dim() != 2 || w.numel() == 0) throw std::invalid_argument("Weight: a matrix with rows and columns");
+  auto r = std::make_shared<Weight>();
+  r->N = w.size(0);
+  r->K = w.size(1);
+  if (transpose) std::tie(r->q, r->s, r->qt, r->st) = quant_both(w, MXFP4_E2M1, MXFP4_ROWS_PI);
+  else std::tie(r->q, r->s) = quant(w, MXFP4_E2M1, MXFP4_ROWS_PI);
+  return r;
+}
+
+// MX(x) [.., K] . MX(W)^T from an operand [N, K] in the PI order
+Tensor product(const Tensor& x, const Tensor& wq, const Tensor& ws, int64_t N, int64_t K, int64_t fmt) {
   const char* what = "mx4_linear";
   gpu(x, what);
   same(x, wq, what);
   const int64_t type = half_type(x, what);
   need(x.dim() >= 1 && x.size(-1) == K, what, "the last dimension is not the weight's input size");
-  c10::OptionalDeviceGuard guard(x.device());
+  const Scope sc(x);
   const Tensor m = rows_of(x);
   const int64_t M = m.size(0);
   Tensor y = empty({M, N}, x.scalar_type(), x);
   if (M > MXFP4_FEW_ROWS) {
     Temp a(M, K, fmt, x);
-    ok(mxfp4_quant(ptr(m), type, M, K, ld_of(m), fmt, a.q, a.s, MXFP4_ROWS_PLAIN, nullptr, nullptr, 0, 0, 0, stm(stream)),
+    ok(mxfp4_quant(ptr(m), type, M, K, ld_of(m), fmt, a.q, a.s, MXFP4_ROWS_PLAIN, nullptr, nullptr, 0, 0, 0, sc.stream),
        "mxfp4_quant");
-    ok(mxfp4_gemm(a.q, a.s, fmt, ptr(wq), ptr(ws), MXFP4_ROWS_PI, M, N, pad(K, 128), ptr(y), N, type, stm(stream)),
+    ok(mxfp4_gemm(a.q, a.s, fmt, ptr(wq), ptr(ws), MXFP4_ROWS_PI, M, N, pad(K, 128), ptr(y), N, type, sc.stream),
        "mxfp4_gemm");
   } else if (M) {
-    ok(mxfp4_few(ptr(m), ld_of(m), fmt, ptr(wq), ptr(ws), M, N, K, ptr(y), N, type, stm(stream)), "mxfp4_few");
+    ok(mxfp4_few(ptr(m), ld_of(m), fmt, ptr(wq), ptr(ws), M, N, K, ptr(y), N, type, sc.stream), "mxfp4_few");
   }
   return shaped(y, x, N);
 }
 
-// h [.., N]; with save also what the backward pass needs
-std::tuple<Tensor, OptT> gated(const Tensor& x, const Tensor& wq, const Tensor& ws, int64_t N, int64_t K, const OptT& add,
-                               int64_t fn, int64_t fmt, bool save, int64_t stream) {
+using torch::autograd::Node;
+using torch::autograd::SavedVariable;
+using torch::autograd::variable_list;
+
+bool records(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+void once(const char* what) {
+  need(!at::GradMode::is_enabled(), what, "the backward pass has no derivative of its own (create_graph)");
+}
+template <class T, class... A>
+std::shared_ptr<T> make_node(A&&... a) {
+  return std::shared_ptr<T>(new T(std::forward<A>(a)...), torch::autograd::deleteNode);
+}
+
+// dx = MX(dy) . MX(W^T)^T.  forward false: a product with the transpose, whose own gradient is one with W.
+struct LinearNode : Node {
+  WeightP w;
+  int64_t fmt;
+  bool forward;
+  LinearNode(WeightP w_, int64_t f, bool fw) : w(std::move(w_)), fmt(f), forward(fw) {}
+  std::string name() const override { return "Mx4Linear"; }
+  variable_list apply(variable_list&& g) override;
+};
+
+Tensor linear(const WeightP& w, const Tensor& x, int64_t fmt, bool forward) {
+  if (!records(x))
+    return forward ? product(x, w->q, w->s, w->N, w->K, fmt) : product(x, w->qt, w->st, w->K, w->N, fmt);
+  if (!w->qt.defined())
+    throw std::invalid_argument("mx4_linear: this weight was made without its transpose, it has no input gradient");
+  Tensor y = forward ? product(x, w->q, w->s, w->N, w->K, fmt) : product(x, w->qt, w->st, w->K, w->N, fmt);
+  auto node = make_node<LinearNode>(w, fmt, forward);
+  node->set_next_edges(torch::autograd::collect_next_edges(x));
+  torch::autograd::set_history(y, node);
+  return y;
+}
+
+variable_list LinearNode::apply(variable_list&& g) {
+  if (!g[0].defined() || !task_should_compute_output(0)) return {Tensor()};
+  return {linear(w, g[0], fmt, !forward)};
+}
+
+// ------------------------------------------------------------------ the gated block
+struct Gated {
+  int64_t N, K;
+  Tensor q, s, qt, st;  // GATE and UP rows along K; [K, 2 pad(N, 128)] along N, rows in the PI order
+};
+using GatedP = std::shared_ptr<Gated>;
+
+GatedP make_gated(const Tensor& wg, const Tensor& wu) {
+  const char* what = "GatedWeight";
+  gpu(wg, what);
+  same(wg, wu, what);
+  need(wg.dim() == 2 && wg.sizes() == wu.sizes() && wg.scalar_type() == wu.scalar_type() && wg.numel() > 0, what,
+       "two matrices of one shape and type");
+  const Scope sc(wg);
+  const int64_t N = wg.size(0), K = wg.size(1), nt = cdiv(N, 128);
+  Operand o = operand(2 * pad(N, 32), K, MXFP4_E2M1, wg), t = operand(K, 2 * nt * 128, MXFP4_E2M1, wg);
+  for (int i = 0; i < 2; ++i) {
+    const Tensor m = rows_of(i ? wu : wg);
+    ok(mxfp4_quant(ptr(m), type_of(m, what), N, K, ld_of(m), MXFP4_E2M1, ptr(o.q), ptr(o.s),
+                   i ? MXFP4_ROWS_UP : MXFP4_ROWS_GATE, ptr(t.q), ptr(t.s), MXFP4_ROWS_PI, i * nt, 2 * nt, sc.stream),
+       "mxfp4_quant");
+  }
+  return std::make_shared<Gated>(Gated{N, K, o.q, o.s, t.q, t.s});
+}
+
+// h [.., N] and, with save, what the backward pass needs
+std::tuple<Tensor, Tensor> gated_forward(const Gated& w, const Tensor& x, const OptT& add, int64_t fn, int64_t fmt,
+                                         bool save) {
   const char* what = "mx4_gated";
-  gpu(x, what);
-  same(x, wq, what);
-  const int64_t type = half_type(x, what);
-  need(x.dim() >= 1 && x.size(-1) == K, what, "the last dimension is not the weight's input size");
-  c10::OptionalDeviceGuard guard(x.device());
+  const int64_t type = half_type(x, what), N = w.N, K = w.K;
+  const Scope sc(x);
   const Tensor m = rows_of(x);
   const int64_t M = m.size(0);
   Tensor ad;
+  int64_t ld_add = 0;
   if (add) {
-    same(x, *add, what);
-    need(add->scalar_type() == x.scalar_type() && add->dim() >= 1 && add->size(-1) == 2 * N, what,
-         "the addend has x's type and 2 N columns");
-    ad = add->dim() == 1 ? add->unsqueeze(0) : rows_of(*add);
-    need(ad.size(0) == M || ad.size(0) == 1, what, "the addend has x's rows, or one");
-    if (ad.stride(1) != 1) ad = ad.contiguous();
+    ad = rows_of(*add);
+    ld_add = M > 1 ? ad.stride(0) : 0;
+    if (ld_add && ld_add < 2 * N) {  // overlapping rows
+      ad = ad.contiguous();
+      ld_add = 2 * N;
+    }
   }
-  const int64_t ld_add = !add || ad.size(0) == 1 ? 0 : ad.stride(0);
-  if (add && ld_add != 0 && ld_add < 2 * N) ad = ad.contiguous();
-  void* pa = add ? ptr(ad) : nullptr;
-  const int64_t la = add && ld_add != 0 ? ad.stride(0) : 0;
-  Tensor h = empty({M, N}, x.scalar_type(), x);
-  OptT gu;
+  const void* pa = add ? ptr(ad) : nullptr;
+  Tensor h = empty({M, N}, x.scalar_type(), x), gu;
   if (save) gu = empty({mxfp4_gated_saved_elems(M, N)}, x.scalar_type(), x);
   if (M > MXFP4_FEW_ROWS || (save && M)) {
     Temp a(M, K, fmt, x);
-    ok(mxfp4_quant(ptr(m), type, M, K, ld_of(m), fmt, a.q, a.s, MXFP4_ROWS_PLAIN, nullptr, nullptr, 0, 0, 0, stm(stream)),
+    ok(mxfp4_quant(ptr(m), type, M, K, ld_of(m), fmt, a.q, a.s, MXFP4_ROWS_PLAIN, nullptr, nullptr, 0, 0, 0, sc.stream),
        "mxfp4_quant");
-    ok(mxfp4_gated(a.q, a.s, fmt, ptr(wq), ptr(ws), M, N, pad(K, 128), pa, la, fn, ptr(h), N, ptr(gu), type, stm(stream)),
+    ok(mxfp4_gated(a.q, a.s, fmt, ptr(w.q), ptr(w.s), M, N, pad(K, 128), pa, ld_add, fn, ptr(h), N,
+                   save ? ptr(gu) : nullptr, type, sc.stream),
        "mxfp4_gated");
   } else if (M) {
-    ok(mxfp4_few_gated(ptr(m), ld_of(m), fmt, ptr(wq), ptr(ws), M, N, K, pa, la, fn, ptr(h), N, type, stm(stream)),
+    ok(mxfp4_few_gated(ptr(m), ld_of(m), fmt, ptr(w.q), ptr(w.s), M, N, K, pa, ld_add, fn, ptr(h), N, type, sc.stream),
        "mxfp4_few_gated");
   }
   return {shaped(h, x, N), gu};
 }
 
-// dx [M, K] and, if wanted, [dg | du] [M, 2 N], from the saved gu and dh [.., N]
-std::tuple<Tensor, OptT> gated_bwd(const Tensor& gu, const Tensor& dh, const Tensor& wtq, const Tensor& wts, int64_t N,
-                                   int64_t K, int64_t fn, int64_t fmt, bool want_dx, bool want_dgu, int64_t stream) {
-  const char* what = "mx4_gated backward";
-  gpu(dh, what);
-  c10::OptionalDeviceGuard guard(dh.device());
-  const int64_t type = half_type(dh, what);
-  Tensor d = rows_of(dh);
-  if (d.size(0) > 1 && d.stride(0) < N) d = d.contiguous();  // a broadcast gradient
-  const int64_t M = d.size(0), C = 2 * pad(N, 128);
-  need(d.size(1) == N && gu.numel() == mxfp4_gated_saved_elems(M, N) && gu.scalar_type() == dh.scalar_type(), what,
-       "dh does not belong to the saved pass");
-  Tensor dx = empty({want_dx ? M : 0, K}, dh.scalar_type(), dh);
-  OptT dgu;
-  if (want_dgu) dgu = empty({M, 2 * N}, dh.scalar_type(), dh);
-  if (M) {
-    Temp a(M, C, fmt, dh);
-    ok(mxfp4_gated_bwd(ptr(gu), ptr(d), ld_of(d), M, N, fn, type, fmt, a.q, a.s, ptr(dgu), stm(stream)), "mxfp4_gated_bwd");
-    if (want_dx)
-      ok(mxfp4_gemm(a.q, a.s, fmt, ptr(wtq), ptr(wts), MXFP4_ROWS_PI, M, K, C, ptr(dx), K, type, stm(stream)), "mxfp4_gemm");
+struct GatedNode : Node {
+  GatedP w;
+  int64_t fn, fmt;
+  std::vector<int64_t> lead;  // x's leading dimensions
+  SavedVariable gu;
+  std::string name() const override { return "Mx4Gated"; }
+  void release_variables() override { gu.reset_data(); }
+  variable_list apply(variable_list&& g) override {
+    const char* what = "mx4_gated";
+    const bool want_dx = task_should_compute_output(0), want_add = num_outputs() > 1 && task_should_compute_output(1);
+    variable_list out(num_outputs());
+    if (!g[0].defined()) return out;
+    once(what);
+    const Tensor saved = gu.unpack(), &dh = g[0];
+    const int64_t N = w->N, K = w->K, C = 2 * pad(N, 128), type = half_type(dh, what);
+    const Scope sc(dh);
+    Tensor d = rows_of(dh);
+    if (d.size(0) > 1 && d.stride(0) < N) d = d.contiguous();  // a broadcast gradient
+    const int64_t M = d.size(0);
+    Tensor dx, dgu;
+    if (want_dx) dx = empty({M, K}, dh.scalar_type(), dh);
+    if (want_add) dgu = empty({M, 2 * N}, dh.scalar_type(), dh);
+    if (M) {
+      Temp a(M, C, fmt, dh);
+      ok(mxfp4_gated_bwd(ptr(saved), ptr(d), ld_of(d), M, N, fn, type, fmt, a.q, a.s, want_add ? ptr(dgu) : nullptr,
+                         sc.stream),
+         "mxfp4_gated_bwd");
+      if (want_dx)
+        ok(mxfp4_gemm(a.q, a.s, fmt, ptr(w->qt), ptr(w->st), MXFP4_ROWS_PI, M, K, C, ptr(dx), K, type, sc.stream),
+           "mxfp4_gemm");
+    }
+    auto shape = lead;
+    shape.push_back(K);
+    if (want_dx) out[0] = dx.view(shape);
+    shape.back() = 2 * N;
+    if (want_add) out[1] = dgu.view(shape);
+    return out;
   }
-  return {dx, dgu};
+};
+
+Tensor gated(const GatedP& w, const Tensor& x, const OptT& add_, int64_t fn, int64_t fmt) {
+  const char* what = "mx4_gated";
+  gpu(x, what);
+  same(x, w->q, what);
+  half_type(x, what);
+  need(x.dim() >= 1 && x.size(-1) == w->K, what, "the last dimension is not the weight's input size");
+  auto lead = x.sizes().vec();
+  OptT add;
+  if (add_) {
+    same(x, *add_, what);
+    need(add_->scalar_type() == x.scalar_type(), what, "the addend has x's type");
+    lead.back() = 2 * w->N;
+    add = add_->expand(lead);  // recorded: the gradient of what is broadcast is summed
+  }
+  lead.pop_back();
+  if (!records(x) && !(add && records(*add))) return std::get<0>(gated_forward(*w, x, add, fn, fmt, false));
+  auto [h, gu] = gated_forward(*w, x, add, fn, fmt, true);
+  auto node = make_node<GatedNode>();
+  node->w = w;
+  node->fn = fn;
+  node->fmt = fmt;
+  node->lead = lead;
+  node->gu = SavedVariable(gu, false);
+  if (add) node->set_next_edges(torch::autograd::collect_next_edges(x, *add));
+  else node->set_next_edges(torch::autograd::collect_next_edges(x));
+  torch::autograd::set_history(h, node);
+  return h;
 }
 
-// loss [T], gradient (or none), workspace of the statistics (kept by the autograd form).  stages as in distill_topk_kl.
-std::tuple<OptT, OptT, OptT> topk_kl(const Tensor& z, const Tensor& idx, const Tensor& t, const OptT& weight, double tau,
-                                     const OptT& lse, bool want_loss, bool want_grad, const OptT& out, const OptT& ws_in,
-                                     int64_t stages, int64_t stream) {
+// ------------------------------------------------------------------ distillation
+struct Kl {  // a checked call
+  const Tensor& z;
+  Tensor idx, t, lse;
+  int64_t T, V, k, parts;
+  double tau;
+};
+
+Kl kl_call(const Tensor& z, const Tensor& idx, const Tensor& t, double tau, const OptT& lse) {
   const char* what = "topk_kl";
-  gpu(z, what);
   need(z.dim() == 2 && idx.dim() == 2 && t.dim() == 2 && idx.sizes() == t.sizes() && idx.size(0) == z.size(0), what,
        "logits [T, V] with the teacher's indices and logits [T, k]");
   const int64_t T = z.size(0), V = z.size(1), k = idx.size(1);
   need(V > 0 && k > 0, what, "empty vocabulary or no teacher entries");
   need(z.stride(1) == 1 || V == 1, what, "the logits' columns must be contiguous");
-  need(T <= 1 || z.stride(0) >= V || !out, what, "rows of the logits overlap");
   need(idx.scalar_type() == at::kInt || idx.scalar_type() == at::kLong, what, "32- or 64-bit indices");
   same(z, idx, what);
   same(z, t, what);
-  c10::OptionalDeviceGuard guard(z.device());
-  auto vec = [&](const OptT& v, const char* msg) -> Tensor {
-    if (!v) return Tensor();
-    same(z, *v, what);
-    need(v->dim() == 1 && v->size(0) == T, what, msg);
-    return v->to(at::kFloat).contiguous();
-  };
-  const Tensor w = vec(weight, "one weight a row"), l = vec(lse, "one teacher logsumexp a row");
-  const Tensor id = idx.stride(1) == 1 || k == 1 ? idx : idx.contiguous();
-  Tensor tt = t.to(at::kFloat);
-  if (tt.stride(1) != 1 && k > 1) tt = tt.contiguous();
-  OptT loss, grad, ws = ws_in;
-  if (want_loss) loss = empty({T}, at::kFloat, z);
-  if (want_grad) {
-    if (out) {
-      same(z, *out, what);
-      need(out->dim() == 2 && out->sizes() == z.sizes() && out->scalar_type() == z.scalar_type() &&
-               (out->stride(1) == 1 || V == 1) && (T <= 1 || out->stride(0) >= V),
-           what, "the gradient's buffer has the logits' shape and type and contiguous columns");
-      grad = *out;
+  Kl c{z, idx.stride(1) == 1 || k == 1 ? idx : idx.contiguous(), t.to(at::kFloat), Tensor(), T, V, k, 1, tau};
+  if (c.t.stride(1) != 1 && k > 1) c.t = c.t.contiguous();
+  if (lse) {
+    same(z, *lse, what);
+    need(lse->dim() == 1 && lse->size(0) == T, what, "one teacher logsumexp a row");
+    c.lse = lse->to(at::kFloat).contiguous();
+  }
+  c.parts = distill_parts(T, V);
+  return c;
+}
+
+void kl_run(const Kl& c, const Tensor& weight, const Tensor& loss, const Tensor& grad, const Tensor& ws, int64_t stages,
+            void* stream) {
+  if (!c.T) return;
+  auto f = [](const Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; };
+  const bool one = c.T == 1;
+  ok(distill_topk_kl(ptr(c.z), type_of(c.z, "topk_kl"), one ? c.V : c.z.stride(0), c.T, c.V, ptr(c.idx),
+                     c.idx.element_size(), one ? c.k : c.idx.stride(0), f(c.t), one ? c.k : c.t.stride(0), c.k, (float)c.tau,
+                     f(c.lse), f(weight), f(loss), grad.defined() ? ptr(grad) : nullptr,
+                     !grad.defined() ? 0 : one ? c.V : grad.stride(0), c.parts, stages, ws.defined() ? ptr(ws) : nullptr,
+                     stream),
+     "distill_topk_kl");
+}
+Tensor kl_workspace(const Kl& c) { return empty({distill_workspace_size(c.T, c.k, c.parts)}, at::kByte, c.z); }
+Tensor row_weight(const Kl& c, const Tensor& w) {
+  same(c.z, w, "topk_kl");
+  need(w.dim() == 1 && w.size(0) == c.T, "topk_kl", "one weight a row");
+  return w.to(at::kFloat).contiguous();
+}
+
+std::tuple<Tensor, Tensor> topk_kl_rows(const Tensor& z, const Tensor& idx, const Tensor& t, const OptT& weight, double tau,
+                                        const OptT& lse, const OptT& out) {
+  const char* what = "topk_kl_rows";
+  gpu(z, what);
+  const Scope sc(z);
+  const Kl c = kl_call(z, idx, t, tau, lse);
+  Tensor w, grad, ws;
+  if (weight) w = row_weight(c, *weight);
+  if (out) {
+    same(z, *out, what);
+    need(out->dim() == 2 && out->sizes() == z.sizes() && out->scalar_type() == z.scalar_type() &&
+             (out->stride(1) == 1 || c.V == 1) && (c.T <= 1 || out->stride(0) >= c.V),
+         what, "the gradient's buffer has the logits' shape and type, contiguous columns and rows that do not overlap");
+    grad = *out;
+  } else {
+    grad = empty({c.T, c.V}, z.scalar_type(), z);
+  }
+  Tensor loss = empty({c.T}, at::kFloat, z);
+  if (c.parts > 1) ws = kl_workspace(c);
+  kl_run(c, w, loss, grad, ws, DISTILL_STATS | DISTILL_FINISH, sc.stream);
+  return {loss, grad};
+}
+
+struct KlNode : Node {
+  SavedVariable z, idx, t, lse, ws;
+  bool has_lse;
+  double tau;
+  std::string name() const override { return "TopkKl"; }
+  void release_variables() override {
+    for (SavedVariable* v : {&z, &idx, &t, &lse, &ws}) v->reset_data();
+  }
+  variable_list apply(variable_list&& g) override {
+    if (!g[0].defined() || !task_should_compute_output(0)) return {Tensor()};
+    once("topk_kl");
+    const Tensor zz = z.unpack(), ii = idx.unpack(), tt = t.unpack(), w0 = ws.unpack();
+    const OptT ll = has_lse ? OptT(lse.unpack()) : OptT();
+    const Scope sc(zz);
+    const Kl c = kl_call(zz, ii, tt, tau, ll);
+    Tensor grad = empty({c.T, c.V}, zz.scalar_type(), zz);
+    kl_run(c, row_weight(c, g[0]), Tensor(), grad, w0, DISTILL_FINISH, sc.stream);
+    return {grad};
+  }
+};
+
+Tensor topk_kl(const Tensor& z, const Tensor& idx, const Tensor& t, double tau, const OptT& lse) {
+  gpu(z, "topk_kl");
+  const bool rec = records(z);
+  Tensor loss, ws;
+  {
+    const Scope sc(z);
+    const Kl c = kl_call(z, idx, t, tau, lse);
+    loss = empty({c.T}, at::kFloat, z);
+    if (c.parts > 1 || rec) ws = kl_workspace(c);
+    if (rec) {  // the statistics are kept
+      kl_run(c, Tensor(), Tensor(), Tensor(), ws, DISTILL_STATS, sc.stream);
+      kl_run(c, Tensor(), loss, Tensor(), ws, DISTILL_FINISH, sc.stream);
     } else {
-      grad = empty({T, V}, z.scalar_type(), z);
+      kl_run(c, Tensor(), loss, Tensor(), ws, DISTILL_STATS | DISTILL_FINISH, sc.stream);
     }
   }
-  // the loss alone reads the logits once and is split the same; statistics that are kept always go through ws
-  const int64_t parts = distill_parts(T, V, lse.has_value());
-  if (T && !ws && (parts > 1 || stages != 3))
-    ws = empty({distill_workspace_size(T, k, parts)}, at::kByte, z);
-  if (T)
-    ok(distill_topk_kl(ptr(z), type_of(z, what), T <= 1 ? V : z.stride(0), T, V, ptr(id), id.element_size(),
-                       T <= 1 ? k : id.stride(0), tt.data_ptr<float>(), T <= 1 ? k : tt.stride(0), k, (float)tau,
-                       l.defined() ? l.data_ptr<float>() : nullptr, w.defined() ? w.data_ptr<float>() : nullptr,
-                       loss ? loss->data_ptr<float>() : nullptr, ptr(grad), grad ? (T <= 1 ? V : grad->stride(0)) : 0, parts,
-                       stages, ptr(ws), stm(stream)),
-       "distill_topk_kl");
-  return {loss, grad, ws};
+  if (!rec) return loss;
+  auto node = make_node<KlNode>();
+  node->z = SavedVariable(z, false);
+  node->idx = SavedVariable(idx, false);
+  node->t = SavedVariable(t.detach(), false);
+  if (lse) node->lse = SavedVariable(lse->detach(), false);
+  node->ws = SavedVariable(ws, false);
+  node->has_lse = lse.has_value();
+  node->tau = tau;
+  node->set_next_edges(torch::autograd::collect_next_edges(z));
+  torch::autograd::set_history(loss, node);
+  return loss;
 }
 
 }  // namespace
@@ -328,15 +514,26 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     g_error = e.ptr();
   });
   m.def("abi_version", [] { return (int64_t)MXFP4_OPS_ABI_VERSION; });
-  m.def("code_bytes", &code_bytes);
-  m.def("scale_bytes", &scale_bytes);
+  py::class_<Weight, WeightP>(m, "Weight")
+      .def(py::init(&make_weight), Free())
+      .def_readonly("N", &Weight::N)
+      .def_readonly("K", &Weight::K)
+      .def_property_readonly("nbytes", [](const Weight& w) {
+        return w.q.nbytes() + w.s.nbytes() + (w.qt.defined() ? w.qt.nbytes() + w.st.nbytes() : 0);
+      });
+  py::class_<Gated, GatedP>(m, "Gated")
+      .def(py::init(&make_gated), Free())
+      .def_readonly("N", &Gated::N)
+      .def_readonly("K", &Gated::K)
+      .def_property_readonly("nbytes", [](const Gated& w) {
+        return w.q.nbytes() + w.s.nbytes() + w.qt.nbytes() + w.st.nbytes();
+      });
   m.def("quant", &quant, Free());
   m.def("quant_both", &quant_both, Free());
-  m.def("quant_gate_up", &quant_gate_up, Free());
   m.def("dequant", &dequant, Free());
   m.def("gemm", &gemm, Free());
-  m.def("linear", &linear, Free());
+  m.def("linear", [](const WeightP& w, const Tensor& x, int64_t fmt) { return linear(w, x, fmt, true); }, Free());
   m.def("gated", &gated, Free());
-  m.def("gated_bwd", &gated_bwd, Free());
+  m.def("topk_kl_rows", &topk_kl_rows, Free());
   m.def("topk_kl", &topk_kl, Free());
 }

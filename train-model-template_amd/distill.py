@@ -15,48 +15,17 @@ loss and gradient 0, whatever its logits hold; so has the gradient of a row of w
 twice in p and once in q.  Logits of -inf have q = 0: a teacher entry there makes the loss infinite.  A row whose logits
 are all -inf has gradient 0.  NaN logits make their row NaN.
 """
-import torch
-
 import _native
-
-_STATS, _FINISH = 1, 2
 
 
 def topk_kl_rows(logits, teacher_idx, teacher_logits, weight=None, temperature=1.0, teacher_lse=None, out=None):
     """(loss [T] fp32, d(Σ weight · loss) / d logits [T, V]) in one call, for a training step that knows its rows' weights.
     logits [T, V] bf16, f16 or f32, contiguous columns; teacher_idx [T, k] int32 or int64, teacher_logits [T, k], k <=
     1024; weight [T] or None for 1.  The gradient goes to `out` (which may be the logits), else to a new tensor."""
-    loss, grad, _ = _native.host4().topk_kl(logits.detach(), teacher_idx, teacher_logits, weight, temperature, teacher_lse,
-                                            True, True, out, None, _STATS | _FINISH,
-                                            _native.stream_of(logits, "topk_kl_rows"))
-    return loss, grad
-
-
-class _TopkKL(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, idx, t, temperature, lse):
-        st = _native.stream_of(logits, "topk_kl")
-        h = _native.host4()
-        _, _, ws = h.topk_kl(logits, idx, t, None, temperature, lse, False, False, None, None, _STATS, st)
-        loss, _, _ = h.topk_kl(logits, idx, t, None, temperature, lse, True, False, None, ws, _FINISH, st)
-        ctx.save_for_backward(logits, idx, t, lse, ws)
-        ctx.temperature = temperature
-        return loss
-
-    @staticmethod
-    def backward(ctx, dloss):
-        logits, idx, t, lse, ws = ctx.saved_tensors
-        _, grad, _ = _native.host4().topk_kl(logits, idx, t, dloss, ctx.temperature, lse, False, True, None, ws, _FINISH,
-                                             _native.stream_of(logits, "topk_kl"))
-        return grad, None, None, None, None
+    return _native.host4().topk_kl_rows(logits, teacher_idx, teacher_logits, weight, temperature, teacher_lse, out)
 
 
 def topk_kl(logits, teacher_idx, teacher_logits, temperature=1.0, teacher_lse=None):
     """The loss of every row, [T] fp32, differentiable with respect to the logits (the statistics of the forward pass are
     kept, so that the backward pass reads the logits once).  The teacher's side has no gradient."""
-    teacher_logits = teacher_logits.detach()
-    teacher_lse = None if teacher_lse is None else teacher_lse.detach()
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return _TopkKL.apply(logits, teacher_idx, teacher_logits, temperature, teacher_lse)
-    return _native.host4().topk_kl(logits, teacher_idx, teacher_logits, None, temperature, teacher_lse, True, False, None,
-                                   None, _STATS | _FINISH, _native.stream_of(logits, "topk_kl"))[0]
+    return _native.host4().topk_kl(logits, teacher_idx, teacher_logits, temperature, teacher_lse)
