@@ -8,8 +8,9 @@
  *   C is padded with zeros to Cp = ceil(C / 128) * 128; rows are padded to Rp = ceil(R / 32) * 32 (contents of the padded
  *   rows are undefined).
  *   E2M1 codes: blocks of 16 rows x 128 codes, 1 KB each, block (r / 16, c / 128) at ((r / 16) * (Cp / 128) + c / 128) *
- *     1024; in a block row r % 16 takes 64 bytes whose 16-byte chunk k (codes 32 k ..) sits at position k ^ ((r >> 2) & 3);
- *     the code of an even column is the low half of its byte.  Rp * Cp / 2 bytes.
+ *     1024; a block holds its first 64 columns, then the others, 512 bytes each, in which row r % 16 takes 32 bytes whose
+ *     16-byte chunk k (codes 32 k ..) sits at position k ^ ((r >> 3) & 1) (so 16 rows' reads of one chunk meet every LDS
+ *     bank); the code of an even column is the low half of its byte.  Rp * Cp / 2 bytes.
  *   E4M3 codes: the MX-tiled layout of mxfp8_mlp.h (blocks of 16 rows x 64 codes).  Rp * Cp bytes.
  *   Scales: the 128x4 blocked layout of mxfp8_mlp.h, ceil(R / 128) * (Cp / 128) * 512 bytes.
  * Row orders of a weight operand: MXFP4_ROWS_PLAIN; MXFP4_ROWS_PI: inside each 32-row block position a holds row

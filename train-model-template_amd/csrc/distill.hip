@@ -319,7 +319,7 @@ void distill_kernel(const Args a) {
       unpack_vec<kT>(raw, x);
 #pragma unroll
       for (int i = 0; i < n; ++i) x[i] = value(x[i]);
-      *reinterpret_cast<uint4*>(gp + (uint32_t)v * 16u) = pack_vec<kT>(x);
+      store_codes<true>(reinterpret_cast<uint8_t*>(gp + (uint32_t)v * 16u), pack_vec<kT>(x));
     };
     if constexpr (kHold > 0) {
 #pragma unroll

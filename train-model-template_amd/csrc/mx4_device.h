@@ -93,12 +93,131 @@ __device__ __forceinline__ uint32_t absmax8(const float* v) {
   return m;
 }
 
+// ---- groups of eight values as they are loaded: 16-bit types packed in one uint4, fp32 in two
+template <int kT>
+struct Group {
+  uint4 w;
+  __device__ __forceinline__ void values(float* v) const {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (kT == MXFP4_BF16) {
+        v[2 * i] = bf16_lo(u[i]);
+        v[2 * i + 1] = bf16_hi(u[i]);
+      } else {
+        const f16x2 h = __builtin_bit_cast(f16x2, u[i]);
+        v[2 * i] = (float)h[0];
+        v[2 * i + 1] = (float)h[1];
+      }
+    }
+  }
+  // the largest magnitude, as fp32 bits (16-bit patterns without the sign order like magnitudes, NaN on top)
+  __device__ __forceinline__ uint32_t absmax() const {
+    u16x2 m = {0, 0};
+    m = absmax2(absmax2(absmax2(absmax2(m, w.x), w.y), w.z), w.w);
+    const uint32_t b = max(m.x, m.y);
+    if constexpr (kT == MXFP4_BF16) return b << 16;
+    else return abs_bits((float)__builtin_bit_cast(_Float16, (uint16_t)b));
+  }
+};
+template <>
+struct Group<MXFP4_F32> {
+  uint4 w, x;
+  __device__ __forceinline__ void values(float* v) const {
+    const uint32_t u[8] = {w.x, w.y, w.z, w.w, x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(u[i]);
+  }
+  __device__ __forceinline__ uint32_t absmax() const {
+    float v[8];
+    values(v);
+    return absmax8(v);
+  }
+};
+
+// Codes of a group with the block exponent e, as encode8; 16-bit values convert packed, as they are
+template <int kT, int kFmt>
+__device__ __forceinline__ void encode_group(const Group<kT>& g, uint32_t e, uint32_t* r) {
+  if constexpr (kT == MXFP4_F32) {
+    float v[8];
+    g.values(v);
+    encode8<kFmt>(v, e, r);
+  } else {
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(e >= 254u) != 0, 0)) {
+      float v[8];
+      g.values(v);
+      encode8<kFmt>(v, e, r);
+      return;
+    }
+    const float sc = block_scale<kFmt>(e);
+    const uint32_t u[4] = {g.w.x, g.w.y, g.w.z, g.w.w};
+    if constexpr (kFmt == MXFP4_E4M3) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        s16x2 c = {0, 0};
+        if constexpr (kT == MXFP4_BF16) {
+          c = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(c, __builtin_bit_cast(bf16x2, u[2 * i]), sc, false);
+          c = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(c, __builtin_bit_cast(bf16x2, u[2 * i + 1]), sc, true);
+        } else {
+          c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(c, __builtin_bit_cast(f16x2, u[2 * i]), sc, false);
+          c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(c, __builtin_bit_cast(f16x2, u[2 * i + 1]), sc, true);
+        }
+        r[i] = __builtin_bit_cast(uint32_t, c);
+      }
+    } else {
+      uint32_t c = 0;
+      if constexpr (kT == MXFP4_BF16) {
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2, u[0]), sc, 0);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2, u[1]), sc, 1);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2, u[2]), sc, 2);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2, u[3]), sc, 3);
+      } else {
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, __builtin_bit_cast(f16x2, u[0]), sc, 0);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, __builtin_bit_cast(f16x2, u[1]), sc, 1);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, __builtin_bit_cast(f16x2, u[2]), sc, 2);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, __builtin_bit_cast(f16x2, u[3]), sc, 3);
+      }
+      r[0] = c;
+    }
+  }
+}
+
+// A group at p (aligned to 16 bytes), or element by element with zeros past the row's end
+template <int kT, class T>
+__device__ __forceinline__ Group<kT> load_group(const T* p) {
+  Group<kT> g;
+  g.w = *reinterpret_cast<const uint4*>(p);
+  if constexpr (kT == MXFP4_F32) g.x = *reinterpret_cast<const uint4*>(p + 4);
+  return g;
+}
+template <int kT, class T>
+__device__ __forceinline__ Group<kT> load_group_edge(const T* row, int64_t c, int64_t cols) {
+  uint32_t u[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const T t = row[min(c + i, cols - 1)];
+    uint32_t b;
+    if constexpr (kT == MXFP4_F32) b = __builtin_bit_cast(uint32_t, t);
+    else b = __builtin_bit_cast(uint16_t, t);
+    u[i] = c + i < cols ? b : 0u;
+  }
+  Group<kT> g;
+  if constexpr (kT == MXFP4_F32) {
+    g.w = make_uint4(u[0], u[1], u[2], u[3]);
+    g.x = make_uint4(u[4], u[5], u[6], u[7]);
+  } else {
+    g.w = make_uint4(u[0] | u[1] << 16, u[2] | u[3] << 16, u[4] | u[5] << 16, u[6] | u[7] << 16);
+  }
+  return g;
+}
+
 // ---- layouts
 // Byte of code (r, c) in an operand with ct column tiles (128 wide): E2M1 (the code's byte; odd c is its high half) or E4M3
 template <int kFmt>
 __device__ __forceinline__ int64_t code_offset(int64_t r, int64_t c, int64_t ct) {
   if constexpr (kFmt == MXFP4_E4M3) return tiled_offset(r, c, ct * 128);
-  return ((r >> 4) * ct + (c >> 7)) * 1024 + (r & 15) * 64 + ((((c >> 5) & 3) ^ ((r >> 2) & 3)) << 4) + ((c & 31) >> 1);
+  return ((r >> 4) * ct + (c >> 7)) * 1024 + ((c >> 6) & 1) * 512 + (r & 15) * 32 +
+         ((((c >> 5) & 1) ^ ((r >> 3) & 1)) << 4) + ((c & 31) >> 1);
 }
 
 // Position of row r in a row order
@@ -209,7 +328,7 @@ __device__ __forceinline__ void store_run(typename Elem<kT>::T* p, int64_t c, in
 // silu(g) = g s, s = 1 / (1 + exp(-g)); silu' = s (1 + g (1 - s)).
 // gelu(g) = g s(2 c (g + a g^3)) with c = sqrt(2 / pi), a = 0.044715 (0.5 (1 + tanh t) = sigmoid(2 t)), so
 // gelu' = s + g s (1 - s) 2 c (1 + 3 a g^2).  Both with the hardware exp2 and reciprocal, 1 ulp each.
-// s (1 - s) as s times sigmoid(-t), which keeps its relative accuracy for large t.
+// 1 - s is off by 2^-24 where s is near 1, which g (1 - s) + 1 takes as g 2^-24.
 template <int kFn>
 __device__ __forceinline__ float gate_fn(float g) {
   if constexpr (kFn == MXFP4_SILU) {
@@ -223,13 +342,13 @@ template <int kFn>
 __device__ __forceinline__ float gate_fn(float g, float& df) {
   if constexpr (kFn == MXFP4_SILU) {
     const float s = fast_sigmoid(g);
-    df = s * __builtin_fmaf(g, fast_sigmoid(-g), 1.f);
+    df = s * __builtin_fmaf(g, 1.f - s, 1.f);
     return g * s;
   } else {
     const float q = 0.044715f * g * g;
     const float t = 1.5957691216057308f * g * (1.f + q);
     const float s = fast_sigmoid(t);
-    df = s * __builtin_fmaf(g * 1.5957691216057308f * __builtin_fmaf(3.f, q, 1.f), fast_sigmoid(-t), 1.f);
+    df = s * __builtin_fmaf(g * 1.5957691216057308f * __builtin_fmaf(3.f, q, 1.f), 1.f - s, 1.f);
     return g * s;
   }
 }

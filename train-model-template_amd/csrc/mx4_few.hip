@@ -29,53 +29,24 @@ struct FewArgs {
   int fn, vec_x, vec_c;
 };
 
-// 16 values (packed pairs) of columns k.. of a row; zeros past K
+// 16 values of columns k.. of a row, zeros past K
 template <int kT>
-__device__ __forceinline__ void load16p(const uint16_t* row, int k, int K, bool vec, uint32_t* w) {
+__device__ __forceinline__ void load16p(const typename Elem<kT>::T* row, int k, int K, bool vec, Group<kT>* w) {
   if (vec && k + 16 <= K) {
-    const uint4 a = *reinterpret_cast<const uint4*>(row + k), b = *reinterpret_cast<const uint4*>(row + k + 8);
-    w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
-    w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+    w[0] = load_group<kT>(row + k);
+    w[1] = load_group<kT>(row + k + 8);
   } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t lo = k + 2 * i < K ? row[k + 2 * i] : 0, up = k + 2 * i + 1 < K ? row[k + 2 * i + 1] : 0;
-      w[i] = lo | (up << 16);
-    }
-  }
-}
-
-// magnitude bits of the largest of 16 packed values, as of an fp32 value (16-bit patterns order like magnitudes)
-template <int kT>
-__device__ __forceinline__ uint32_t absmax16p(const uint32_t* w) {
-  u16x2 m = {0, 0};
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m = absmax2(m, w[i]);
-  const uint32_t b = max(m.x, m.y);
-  if constexpr (kT == MXFP4_BF16) return b << 16;
-  return abs_bits((float)__builtin_bit_cast(_Float16, (uint16_t)b));
-}
-
-template <int kT>
-__device__ __forceinline__ void unpack16(const uint32_t* w, float* v) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if constexpr (kT == MXFP4_BF16) {
-      v[2 * i] = bf16_lo(w[i]);
-      v[2 * i + 1] = bf16_hi(w[i]);
-    } else {
-      const f16x2 h = __builtin_bit_cast(f16x2, w[i]);
-      v[2 * i] = (float)h[0];
-      v[2 * i + 1] = (float)h[1];
-    }
+    w[0] = load_group_edge<kT>(row, k, K);
+    w[1] = load_group_edge<kT>(row, k + 8, K);
   }
 }
 
 // The lane's operand of one K tile from its 32 values w (E2M1: columns 32 g ..; E4M3: 16 g .. and 64 + 16 g ..), and the
 // scale byte that the instruction reads from this lane (32-block g of its token)
 template <int kT, int kFmt>
-__device__ __forceinline__ v8i operand(const uint32_t* w, int g, uint32_t& scale) {
-  uint32_t a0 = absmax16p<kT>(w), a1 = absmax16p<kT>(w + 8), p, q, e0, e1;
+__device__ __forceinline__ v8i operand(const Group<kT>* w, int g, uint32_t& scale) {
+  const uint32_t a0 = max(w[0].absmax(), w[1].absmax()), a1 = max(w[2].absmax(), w[3].absmax());
+  uint32_t p, q, e0, e1;
   if constexpr (kFmt == MXFP4_E4M3) {
     pair16(a0, p, q);
     e0 = block_exponent<kFmt>(max(p, q));  // block g / 2
@@ -88,22 +59,16 @@ __device__ __forceinline__ v8i operand(const uint32_t* w, int g, uint32_t& scale
   } else {
     e0 = e1 = scale = block_exponent<kFmt>(max(a0, a1));
   }
-  float v[16];
   v8i r = {0, 0, 0, 0, 0, 0, 0, 0};
-  uint32_t c[2], d[2];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    unpack16<kT>(w + 8 * h, v);
-    encode8<kFmt>(v, h ? e1 : e0, c);
-    encode8<kFmt>(v + 8, h ? e1 : e0, d);
+  for (int i = 0; i < 4; ++i) {
+    uint32_t c[2];
+    encode_group<kT, kFmt>(w[i], i < 2 ? e0 : e1, c);
     if constexpr (kFmt == MXFP4_E4M3) {
-      r[4 * h] = (int)c[0];
-      r[4 * h + 1] = (int)c[1];
-      r[4 * h + 2] = (int)d[0];
-      r[4 * h + 3] = (int)d[1];
+      r[2 * i] = (int)c[0];
+      r[2 * i + 1] = (int)c[1];
     } else {
-      r[2 * h] = (int)c[0];
-      r[2 * h + 1] = (int)d[0];
+      r[i] = (int)c[0];
     }
   }
   return r;
@@ -130,18 +95,19 @@ __global__ __launch_bounds__(64 * kWaves) void few_kernel(const FewArgs a) {
   const uint8_t* sp[kB];
 #pragma unroll
   for (int i = 0; i < kB; ++i) {
-    wp[i] = a.b + (rb[i] >> 4) * a.kt * 1024 + r16 * 64 + ((g ^ ((r16 >> 2) & 3)) << 4);
+    wp[i] = a.b + (rb[i] >> 4) * a.kt * 1024 + (g >> 1) * 512 + r16 * 32 + (((g & 1) ^ (r16 >> 3)) << 4);
     const int64_t r = rb[i] + r16;
     sp[i] = a.sb + (r >> 7) * a.kt * 512 + (r & 31) * 16 + ((r & 127) >> 5) * 4 + g;
   }
-  const uint16_t* xrow = reinterpret_cast<const uint16_t*>(a.x) + (int64_t)min(r16, a.M - 1) * a.ld_x;
+  const T* xrow = reinterpret_cast<const T*>(a.x) + (int64_t)min(r16, a.M - 1) * a.ld_x;
   const int k0 = kFmt == MXFP4_E4M3 ? 16 * g : 32 * g, k1 = kFmt == MXFP4_E4M3 ? 64 + 16 * g : 32 * g + 16;
   v4f acc[kB];
 #pragma unroll
   for (int i = 0; i < kB; ++i) acc[i] = v4f{0.f, 0.f, 0.f, 0.f};
   for (int t = t0; t < t1; t += kU) {
     uint4 wv[kU][kB];
-    uint32_t ws[kU][kB], xv[kU][16];
+    uint32_t ws[kU][kB];
+    Group<kT> xv[kU][4];
 #pragma unroll
     for (int u = 0; u < kU; ++u) {  // tiles past the wave's range re-read its last one and are not used
       const int64_t tu = min(t + u, t1 - 1);
@@ -155,7 +121,7 @@ __global__ __launch_bounds__(64 * kWaves) void few_kernel(const FewArgs a) {
     for (int u = 0; u < kU; ++u) {
       const int tu = min(t + u, t1 - 1);
       load16p<kT>(xrow, tu * 128 + k0, a.K, a.vec_x, xv[u]);
-      load16p<kT>(xrow, tu * 128 + k1, a.K, a.vec_x, xv[u] + 8);
+      load16p<kT>(xrow, tu * 128 + k1, a.K, a.vec_x, xv[u] + 2);
     }
 #pragma unroll
     for (int u = 0; u < kU; ++u) {

@@ -14,6 +14,11 @@ namespace {
 
 constexpr int kThreads = 256;
 
+__device__ __forceinline__ uint4 load_nt(const void* p) {
+  const u32x4v v = __builtin_nontemporal_load(reinterpret_cast<const u32x4v*>(p));
+  return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
 struct BwdArgs {
   const void* gu;
   const void* dh;
@@ -25,10 +30,10 @@ struct BwdArgs {
   int vec_dh, vec_dgu;
 };
 
-// 16 codes of v (its other 16 in lane l ^ 32) at row m, column c of an operand with ct column tiles; scale 0 past the rows
+// 16 codes of v (its other 16 in lane l ^ 32) at row m, column c of an operand with ct column tiles; returns the scale byte,
+// 0 past the rows
 template <int kFmt>
-__device__ __forceinline__ void quant_store(const float* v, int64_t m, int64_t c, int64_t ct, bool live, uint8_t* q,
-                                            uint8_t* s, int lane) {
+__device__ __forceinline__ uint32_t quant_store(const float* v, int64_t m, int64_t c, int64_t ct, bool live, uint8_t* q) {
   uint32_t a, b;
   pair32(max(absmax8(v), absmax8(v + 8)), a, b);
   const uint32_t e = block_exponent<kFmt>(max(a, b));
@@ -40,7 +45,7 @@ __device__ __forceinline__ void quant_store(const float* v, int64_t m, int64_t c
     if constexpr (kFmt == MXFP4_E4M3) *reinterpret_cast<uint4*>(p) = make_uint4(c0[0], c0[1], c1[0], c1[1]);
     else *reinterpret_cast<uint2*>(p) = make_uint2(c0[0], c1[0]);
   }
-  if (lane < 32) s[blocked_offset(m, c >> 5, ct)] = live ? (uint8_t)e : (uint8_t)0;
+  return live ? e : 0u;
 }
 
 template <int kT, int kFn, int kFmt>
@@ -51,48 +56,68 @@ __global__ __launch_bounds__(kThreads) void gate_bwd_kernel(const BwdArgs a) {
   const int64_t m = (int64_t)blockIdx.y * 128 + w * 32 + (lane & 31);  // scale bytes of a tile's 128 rows are all written
   const int64_t mc = min(m, (int64_t)a.M - 1);
   const bool live = m < a.M;
+  uint32_t sg = 0, su = 0;  // the row's four scale bytes of the gate's and the up's tile
+  const T* const sv = reinterpret_cast<const T*>(a.gu);
+  const T* const p = reinterpret_cast<const T*>(a.dh) + mc * a.ld_dh;
+  struct Raw {
+    Group<kT> g[2], u[2], d[2];
+  };
+  // a block's values, asked for while the block before is computed; saved values are read once and pass the caches by
+  auto load = [&](int b) {
+    Raw r;
+    const int64_t cb = min((int64_t)blockIdx.x * 128 + b * 32, (nblk - 1) * 32), c = cb + hi * 16;
+    const T* s = sv + saved_offset(mc, c, nblk);
+    r.g[0].w = load_nt(s);
+    r.g[1].w = load_nt(s + 512);
+    r.u[0].w = load_nt(s + 1024);
+    r.u[1].w = load_nt(s + 1536);
+    if (a.vec_dh && cb + 32 <= a.N) {
+      r.d[0] = load_group<kT>(p + c);
+      r.d[1] = load_group<kT>(p + c + 8);
+    } else {
+      r.d[0] = load_group_edge<kT>(p, c, a.N);
+      r.d[1] = load_group_edge<kT>(p, c + 8, a.N);
+    }
+    return r;
+  };
+  Raw cur = load(0);
 #pragma unroll
   for (int b = 0; b < 4; ++b) {
     const int64_t cb = (int64_t)blockIdx.x * 128 + b * 32, c = cb + hi * 16;
+    const Raw raw = cur;
+    if (b < 3) cur = load(b + 1);
     float dg[16], du[16];
-    if (cb < a.N) {
-      float g[16], u[16], d[16];
-      const T* s = reinterpret_cast<const T*>(a.gu) + saved_offset(mc, c, nblk);
-      load8<kT>(s, g);
-      load8<kT>(s + 512, g + 8);
-      load8<kT>(s + 1024, u);
-      load8<kT>(s + 1536, u + 8);
-      const T* p = reinterpret_cast<const T*>(a.dh) + mc * a.ld_dh;
-      if (a.vec_dh && cb + 32 <= a.N) {
-        load8<kT>(p + c, d);
-        load8<kT>(p + c + 8, d + 8);
-      } else {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const T t = p[min(c + i, (int64_t)a.N - 1)];
-          d[i] = Elem<kT>::get(t);
-        }
-      }
+    for (int h = 0; h < 2; ++h) {
+      float g[8], u[8], d[8];
+      raw.g[h].values(g);
+      raw.u[h].values(u);
+      raw.d[h].values(d);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
+      for (int i = 0; i < 8; ++i) {
         float df;
         const float f = gate_fn<kFn>(g[i], df);
-        // the saved values past the last column are undefined
-        dg[i] = c + i < a.N ? d[i] * u[i] * df : 0.f;
-        du[i] = c + i < a.N ? d[i] * f : 0.f;
+        dg[8 * h + i] = d[i] * u[i] * df;
+        du[8 * h + i] = d[i] * f;
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) dg[i] = du[i] = 0.f;
     }
-    quant_store<kFmt>(dg, m, c, 2 * tiles, live, a.q, a.s, lane);
-    quant_store<kFmt>(du, m, tiles * 128 + c, 2 * tiles, live, a.q, a.s, lane);
+    if (cb + 32 > a.N) {  // the saved values past the last column are undefined
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        dg[i] = c + i < a.N ? dg[i] : 0.f;
+        du[i] = c + i < a.N ? du[i] : 0.f;
+      }
+    }
+    sg |= quant_store<kFmt>(dg, m, c, 2 * tiles, live, a.q) << (8 * b);
+    su |= quant_store<kFmt>(du, m, tiles * 128 + c, 2 * tiles, live, a.q) << (8 * b);
     if (a.dgu && live) {
       T* o = reinterpret_cast<T*>(a.dgu) + m * 2 * a.N;
       store_run<kT, 16>(o, c, a.N, a.vec_dgu, dg);
       store_run<kT, 16>(o + a.N, c, a.N, a.vec_dgu, du);
     }
   }
+  const int64_t t = (int64_t)blockIdx.y * 2 * tiles + blockIdx.x + (hi ? tiles : 0);
+  *reinterpret_cast<uint32_t*>(a.s + t * 512 + (lane & 31) * 16 + w * 4) = hi ? su : sg;
 }
 
 template <int kT, int kFn>

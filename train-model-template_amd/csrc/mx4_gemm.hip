@@ -19,15 +19,15 @@ using namespace mx4;
 
 namespace {
 
-template <int kAF_, int kMB_, int kNB_, int kWM_, int kWN_, int kStages_>
+template <int kAF_, int kMB_, int kNB_, int kWM_, int kWN_, int kKS_, int kStages_>
 struct Shape {
-  static constexpr int kAF = kAF_, kMB = kMB_, kNB = kNB_, kWM = kWM_, kWN = kWN_, kStages = kStages_;
+  static constexpr int kAF = kAF_, kMB = kMB_, kNB = kNB_, kWM = kWM_, kWN = kWN_, kKS = kKS_, kStages = kStages_;
   static constexpr int kWaves = kWM * kWN, kThreads = 64 * kWaves;
   static constexpr int kBM = 32 * kMB * kWM, kBN = 32 * kNB * kWN;
   static constexpr int kGroupM = 1024 / kBM;                                      // M-tiles of a tile group
   static constexpr int kTilesA = (kBM + 127) / 128, kTilesB = (kBN + 127) / 128;  // scale tiles of a stage
-  static constexpr int kHalvesA = kAF == MXFP4_E4M3 ? 2 : 1;                      // 64-code blocks of a K tile (E4M3)
-  static constexpr int kBytesA = kBM * 64 * kHalvesA, kBytesB = kBN * 64;
+  static constexpr int kRowA = kAF == MXFP4_E4M3 ? 64 : 32, kRowB = 32;           // bytes of 64 codes of a row
+  static constexpr int kBytesA = kBM * kRowA * kKS, kBytesB = kBN * kRowB * kKS;
   static constexpr int kOffB = kBytesA, kOffS = kOffB + kBytesB, kOffSB = kOffS + kTilesA * 512;
   static constexpr int kStageBytes = kOffS + (kTilesA + kTilesB) * 512;
   // DMAs of a wave and stage: 1 KB slices of A and B, 256-byte pieces of the scale tiles (a wave past the last piece
@@ -135,6 +135,15 @@ __device__ __forceinline__ void load_run16(const void* base, int64_t off, int64_
   }
 }
 
+template <int kT>
+__device__ __forceinline__ void store_nt8(typename Elem<kT>::T* p, const float* f) {
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = f[i];
+  store_codes<true>(reinterpret_cast<uint8_t*>(p), make_uint4(round2<kT>(v[0], v[1]), round2<kT>(v[2], v[3]),
+                                                              round2<kT>(v[4], v[5]), round2<kT>(v[6], v[7])));
+}
+
 template <class S, int kT, int kFn>
 __device__ __forceinline__ void store_gated(const GemmArgs& g, int m0, int n0, int lane, const v16f (*acc)[S::kMB]) {
   typedef typename Elem<kT>::T T;
@@ -163,10 +172,11 @@ __device__ __forceinline__ void store_gated(const GemmArgs& g, int m0, int n0, i
       }
       if (g.gu) {
         T* s = reinterpret_cast<T*>(g.gu) + saved_offset(m, c, nblk);
-        store_run<kT, 8>(s, 0, 8, true, gv);
-        store_run<kT, 8>(s + 512, 0, 8, true, gv + 8);
-        store_run<kT, 8>(s + 1024, 0, 8, true, uv);
-        store_run<kT, 8>(s + 1536, 0, 8, true, uv + 8);
+        // read again by the backward pass alone: past the caches, which keep h
+        store_nt8<kT>(s, gv);
+        store_nt8<kT>(s + 512, gv + 8);
+        store_nt8<kT>(s + 1024, uv);
+        store_nt8<kT>(s + 1536, uv + 8);
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) gv[i] = gate_fn<kFn>(gv[i]) * uv[i];
@@ -187,20 +197,31 @@ void gemm_kernel(const GemmArgs g) {
   const int wn = wave / S::kWM, wm = wave % S::kWM;
   const int m0 = mt_ * S::kBM, n0 = nt_ * S::kBN, kt = g.kt;
 
-  // this wave's slices of a stage.  A slice of A (E4M3): block (row block, half) with the halves outermost in LDS.
-  constexpr int kRowsA = S::kBM / 16;
+  // this wave's slices of a stage.  E4M3: a slice is a block of 16 rows x 64 codes (two halves of a K tile: first all rows
+  // of one, then of the other).  E2M1: a block of 16 rows x 128 codes, or with stages of 64 codes the halves of two blocks.
   const int last_a = ((g.M + 31) >> 5) * 2 - 1, last_b = ((g.rows_b + 31) >> 5) * 2 - 1;  // last row block of 16
-  const uint8_t* ga = g.a + (int64_t)(m0 >> 4) * kt * (1024 * S::kHalvesA);
+  constexpr int kRowsA = S::kBM / 16;
+  auto slice4 = [&](int r0, int sl, int last_rb) -> uint32_t {
+    if constexpr (S::kKS == 2) return (uint32_t)((min((r0 >> 4) + sl, last_rb) - (r0 >> 4)) * kt * 1024) + lane * 16;
+    return (uint32_t)((min((r0 >> 4) + 2 * sl + (lane >> 5), last_rb) - (r0 >> 4)) * kt * 1024) + (lane & 31) * 16;
+  };
+  constexpr int kBlkA = S::kAF == MXFP4_E4M3 ? 2048 : 1024;     // bytes of a 16-row K tile
+  constexpr int kStepA = kBlkA * S::kKS / 2, kStepB = 512 * S::kKS;  // of a stage
+  const uint8_t* ga = g.a + (int64_t)(m0 >> 4) * kt * kBlkA;
   const uint8_t* gb = g.b + (int64_t)(n0 >> 4) * kt * 1024;
   uint32_t oa[S::kSA], ob[S::kSB];
 #pragma unroll
   for (int j = 0; j < S::kSA; ++j) {
-    const int sl = wave * S::kSA + j, half = sl / kRowsA, rb = min((m0 >> 4) + sl % kRowsA, last_a) - (m0 >> 4);
-    oa[j] = (uint32_t)((rb * kt * S::kHalvesA + half) * 1024) + lane * 16;
+    const int sl = wave * S::kSA + j;
+    if constexpr (S::kAF == MXFP4_E4M3) {
+      const int half = sl / kRowsA, rb = min((m0 >> 4) + sl % kRowsA, last_a) - (m0 >> 4);
+      oa[j] = (uint32_t)(rb * kt * 2048 + half * 1024) + lane * 16;
+    } else {
+      oa[j] = slice4(m0, sl, last_a);
+    }
   }
 #pragma unroll
-  for (int j = 0; j < S::kSB; ++j)
-    ob[j] = (uint32_t)((min((n0 >> 4) + wave * S::kSB + j, last_b) - (n0 >> 4)) * kt * 1024) + lane * 16;
+  for (int j = 0; j < S::kSB; ++j) ob[j] = slice4(n0, wave * S::kSB + j, last_b);
   const uint8_t* gsp[S::kSS];
   int so[S::kSS];
 #pragma unroll
@@ -212,15 +233,16 @@ void gemm_kernel(const GemmArgs g) {
     so[j] = S::kOffS + pc * 256;
   }
   const uint32_t lds0 = lds_addr(lds);
-  const int last = kt - 1;
-  auto dma = [&](int s, int slot, int d) {  // DMA d of K tile s into ring slot `slot`
+  const int last = (S::kKS == 2 ? kt : 2 * kt) - 1;
+  auto dma = [&](int s, int slot, int d) {  // DMA d of stage s into ring slot `slot`
     const uint32_t st = lds0 + slot * S::kStageBytes;
     if (d < S::kSA)
-      dma16_at(ga + (int64_t)s * (1024 * S::kHalvesA), oa[d], st + (wave * S::kSA + d) * 1024);
+      dma16_at(ga + (int64_t)s * kStepA, oa[d], st + (wave * S::kSA + d) * 1024);
     else if (d < S::kSA + S::kSB)
-      dma16_at(gb + (int64_t)s * 1024, ob[d - S::kSA], st + S::kOffB + (wave * S::kSB + d - S::kSA) * 1024);
+      dma16_at(gb + (int64_t)s * kStepB, ob[d - S::kSA], st + S::kOffB + (wave * S::kSB + d - S::kSA) * 1024);
     else
-      dma4_at(gsp[d - S::kSA - S::kSB] + (int64_t)s * 512, lane * 4, st + so[d - S::kSA - S::kSB]);
+      dma4_at(gsp[d - S::kSA - S::kSB] + (int64_t)(S::kKS == 2 ? s : s >> 1) * 512, lane * 4,
+              st + so[d - S::kSA - S::kSB]);
   };
 
   v16f acc[kNB][kMB];
@@ -229,7 +251,7 @@ void gemm_kernel(const GemmArgs g) {
 #pragma unroll
     for (int j = 0; j < kMB; ++j) acc[i][j] = v16f{};
 
-  const int rl = lane & 31, hi = lane >> 5, sw = (lane >> 2) & 3, sshift = hi * 8;
+  const int rl = lane & 31, hi = lane >> 5, sshift = hi * 8;
   const int rwa = (S::kBM < 128 ? m0 & 127 : 0) + wm * 32 * kMB, rwb = (S::kBN < 128 ? n0 & 127 : 0) + wn * 32 * kNB;
   const int sao = S::kOffS + (rwa >> 7) * 512 + rl * 16 + ((rwa >> 5) & 3) * 4;
   const int sbo = S::kOffSB + (rwb >> 7) * 512 + rl * 16 + ((rwb >> 5) & 3) * 4;
@@ -249,19 +271,23 @@ void gemm_kernel(const GemmArgs g) {
 #pragma unroll
     for (int i = 0; i < kNB; ++i) scb[i] = snb[i] >> sshift;
   };
+  // E2M1: 16 bytes of a row, chunk hi at its place; E4M3: chunks hi and hi + 2 at theirs (tiled_offset in mx_device.h)
+  const int c4 = (hi ^ ((rl >> 3) & 1)) << 4, c8 = (hi ^ ((rl >> 2) & 3)) << 4;
+  auto row4 = [&](int row0, int half) {  // of row row0 + rl, row0 a multiple of 32
+    return ((row0 + rl) >> 4) * (512 * S::kKS) + half * 512 + (rl & 15) * 32 + c4;
+  };
   auto read_frag = [&](int slot, int half, Frags& f, int r) {
     const uint8_t* st = lds + slot * S::kStageBytes;
     if (r < kMB) {
-      const int row = (wm * kMB + r) * 32 + rl;
+      const int row0 = (wm * kMB + r) * 32;
       if constexpr (S::kAF == MXFP4_E4M3) {
-        const uint8_t* p = st + half * (S::kBM * 64) + row * 64;
-        f.a[r] = frag8(p + ((hi ^ sw) << 4), p + (((hi + 2) ^ sw) << 4));
+        const uint8_t* p = st + half * (S::kBM * 64) + (row0 + rl) * 64;
+        f.a[r] = frag8(p + c8, p + (c8 ^ 32));
       } else {
-        f.a[r] = frag4(st + row * 64 + (((2 * half + hi) ^ sw) << 4));
+        f.a[r] = frag4(st + row4(row0, half));
       }
     } else {
-      const int row = (wn * kNB + r - kMB) * 32 + rl;
-      f.b[r - kMB] = frag4(st + S::kOffB + row * 64 + (((2 * half + hi) ^ sw) << 4));
+      f.b[r - kMB] = frag4(st + S::kOffB + row4((wn * kNB + r - kMB) * 32, half));
     }
   };
   auto mma = [&](const Frags& f, int x, auto half) {  // serpentine: one operand stays from each product to the next
@@ -290,30 +316,58 @@ void gemm_kernel(const GemmArgs g) {
   using H0 = std::integral_constant<int, 0>;
   using H1 = std::integral_constant<int, 1>;
 
-  // K tile s frees its ring slot at the barrier in its second half; that half and the first half of tile s + 1 refill it
-  // with tile s + kStages.  So the ring starts with the second part of its last stage still to come.  Tiles past the end
-  // re-load the last one into slots that nothing reads any more: the number in flight is the same at every wait.
-#pragma unroll
-  for (int q = 0; q < S::kStages; ++q)
-#pragma unroll
-    for (int d = 0; d < (q + 1 < S::kStages ? S::kDma : kD0); ++d) dma(min(q, last), q, d);
-  wait_vmcnt<(S::kStages - 2) * S::kDma + kD0>();
-  stage_barrier();
   Frags f0, f1;
-  read_scales(0);
+  int slot = 0;  // ring slot of the stage at hand
+  if constexpr (S::kKS == 2) {
+    // K tile s frees its ring slot at the barrier in its second half; that half and the first half of tile s + 1 refill it
+    // with tile s + kStages.  So the ring starts with the second part of its last stage still to come.  Tiles past the end
+    // re-load the last one into slots that nothing reads any more: the number in flight is the same at every wait.
 #pragma unroll
-  for (int r = 0; r < kReads; ++r) read_frag(0, 0, f0, r);
-  int slot = 0, pslot = S::kStages - 1;  // ring slots of tile s and of the tile before it
-  for (int s = 0; s <= last; ++s) {
-    take_scales();
-    step(f0, f1, slot, 1, min(s - 1 + S::kStages, last), pslot, kD0, S::kDma, H0{});
-    wait_vmcnt<(S::kStages - 2) * S::kDma>();
-    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): this wave's reads of tile s are in registers
+    for (int q = 0; q < S::kStages; ++q)
+#pragma unroll
+      for (int d = 0; d < (q + 1 < S::kStages ? S::kDma : kD0); ++d) dma(min(q, last), q, d);
+    wait_vmcnt<(S::kStages - 2) * S::kDma + kD0>();
     stage_barrier();
-    pslot = slot;
-    slot = slot + 1 == S::kStages ? 0 : slot + 1;
-    read_scales(slot);
-    step(f1, f0, slot, 0, min(s + S::kStages, last), pslot, 0, kD0, H1{});
+    read_scales(0);
+#pragma unroll
+    for (int r = 0; r < kReads; ++r) read_frag(0, 0, f0, r);
+    int pslot = S::kStages - 1;  // of the tile before
+    for (int s = 0; s <= last; ++s) {
+      take_scales();
+      step(f0, f1, slot, 1, min(s - 1 + S::kStages, last), pslot, kD0, S::kDma, H0{});
+      wait_vmcnt<(S::kStages - 2) * S::kDma>();
+      __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): this wave's reads of tile s are in registers
+      stage_barrier();
+      pslot = slot;
+      slot = slot + 1 == S::kStages ? 0 : slot + 1;
+      read_scales(slot);
+      step(f1, f0, slot, 0, min(s + S::kStages, last), pslot, 0, kD0, H1{});
+    }
+  } else {
+    // a barrier a step: its slot is refilled within the step
+#pragma unroll
+    for (int q = 0; q < S::kStages; ++q)
+#pragma unroll
+      for (int d = 0; d < S::kDma; ++d) dma(min(q, last), q, d);
+    wait_vmcnt<(S::kStages - 1) * S::kDma>();
+    stage_barrier();
+    read_scales(0);
+#pragma unroll
+    for (int r = 0; r < kReads; ++r) read_frag(0, 0, f0, r);
+    auto one = [&](int s, Frags& cur, Frags& nxt, auto half) {
+      wait_vmcnt<(S::kStages - 2) * S::kDma>();
+      __builtin_amdgcn_s_waitcnt(0xc07f);
+      stage_barrier();
+      take_scales();
+      const int old = slot;
+      slot = slot + 1 == S::kStages ? 0 : slot + 1;
+      read_scales(slot);
+      step(cur, nxt, slot, 0, min(s + S::kStages, last), old, 0, S::kDma, half);
+    };
+    for (int s = 0; s <= last; s += 2) {
+      one(s, f0, f1, H0{});
+      one(s + 1, f1, f0, H1{});
+    }
   }
   wait_vmcnt<0>();  // the redundant loads land before the workgroup's LDS is given away
 
@@ -334,11 +388,13 @@ void gemm_kernel(const GemmArgs g) {
 }
 
 template <int kAF>
-using Big = Shape<kAF, 2, 4, 4, 2, kAF == MXFP4_E4M3 ? 3 : 4>;
+using Big = Shape<kAF, 2, 4, 4, 2, 2, kAF == MXFP4_E4M3 ? 3 : 4>;  // 256 x 256, 8 waves, one workgroup a CU
 template <int kAF>
-using Mid = Shape<kAF, 2, 2, 2, 2, kAF == MXFP4_E4M3 ? 3 : 4>;
+using Tall = Shape<kAF, 2, 4, 4, 1, kAF == MXFP4_E4M3 ? 1 : 2, 3>;  // 256 x 128, 4 waves, two a CU
 template <int kAF>
-using Low = Shape<kAF, 1, 2, 2, 2, 4>;
+using Mid = Shape<kAF, 2, 2, 2, 2, 2, kAF == MXFP4_E4M3 ? 3 : 4>;  // 128 x 128, 4 waves, two a CU
+template <int kAF>
+using Low = Shape<kAF, 1, 2, 2, 2, 2, 4>;  // 64 x 128, 4 waves, two (three) a CU
 
 template <class S, int kEpi>
 int launch(GemmArgs& g, const char* what, hipStream_t st) {
@@ -346,25 +402,32 @@ int launch(GemmArgs& g, const char* what, hipStream_t st) {
   g.tn = (g.rows_b + S::kBN - 1) / S::kBN;
   MX_CHECK_ARG((int64_t)g.tm * g.tn < (1 << 30), "%s: too large", what);
   // a lane's offset from its tile's first row block is held in 32 bits
-  MX_CHECK_ARG((int64_t)std::max(S::kBM, S::kBN) / 16 * g.kt * 1024 * S::kHalvesA < (1LL << 31), "%s: K too large", what);
+  MX_CHECK_ARG((int64_t)std::max(S::kBM, S::kBN) / 16 * g.kt * 2048 < (1LL << 31), "%s: K too large", what);
   g.per = (g.tm * g.tn + 7) / 8;
   gemm_kernel<S, kEpi><<<8 * g.per, S::kThreads, 0, st>>>(g);
   MX_CHECK_LAUNCH(what);
   return MXFP8_OK;
 }
 
-template <int kEpi>
-int dispatch(GemmArgs& g, int64_t a_fmt, const char* what, hipStream_t st) {
+template <int kEpi, int kAF>
+int dispatch(GemmArgs& g, const char* what, hipStream_t st) {
   const int64_t big = ((int64_t)g.M + 255) / 256 * ((g.rows_b + 255) / 256);
   const int64_t mid = ((int64_t)g.M + 127) / 128 * ((g.rows_b + 127) / 128);
-  if (a_fmt == MXFP4_E4M3) {
-    if (big >= 200) return launch<Big<MXFP4_E4M3>, kEpi>(g, what, st);
-    if (mid >= 256) return launch<Mid<MXFP4_E4M3>, kEpi>(g, what, st);
-    return launch<Low<MXFP4_E4M3>, kEpi>(g, what, st);
+  if (const char* e = getenv("MX4_SHAPE")) {
+    switch (atoi(e)) {
+      case 0: return launch<Big<kAF>, kEpi>(g, what, st);
+      case 1: return launch<Tall<kAF>, kEpi>(g, what, st);
+      case 2: return launch<Mid<kAF>, kEpi>(g, what, st);
+      case 3: return launch<Low<kAF>, kEpi>(g, what, st);
+    }
   }
-  if (big >= 200) return launch<Big<MXFP4_E2M1>, kEpi>(g, what, st);
-  if (mid >= 256) return launch<Mid<MXFP4_E2M1>, kEpi>(g, what, st);
-  return launch<Low<MXFP4_E2M1>, kEpi>(g, what, st);
+  if (big >= 200) return launch<Big<kAF>, kEpi>(g, what, st);
+  if (mid >= 256) return launch<Mid<kAF>, kEpi>(g, what, st);
+  return launch<Low<kAF>, kEpi>(g, what, st);
+}
+template <int kEpi>
+int dispatch(GemmArgs& g, int64_t a_fmt, const char* what, hipStream_t st) {
+  return a_fmt == MXFP4_E4M3 ? dispatch<kEpi, MXFP4_E4M3>(g, what, st) : dispatch<kEpi, MXFP4_E2M1>(g, what, st);
 }
 
 int check_operands(const char* what, const void* a, const void* sa, int64_t a_fmt, const void* b, const void* sb,

@@ -5,9 +5,11 @@
 // One 256-thread workgroup per 128 x 128 tile, which is one 512-byte scale tile of either axis: lane l of wave w (rg =
 // l / 16, ch = l % 16) holds columns 8 ch .. + 7 of rows 32 w + 8 rg + 0..7, so a 32-column block of a row is four
 // neighbouring lanes and a 32-row block of a column is one wave.
-//   Row axis: the four lanes agree on their amax by two DPP moves; eight codes leave as one word (E2M1).
+//   Row axis: the four lanes agree on their amax by two DPP moves.  A wave's 32 rows are two whole blocks of the operand's
+//   layout, which pass through LDS (2 KB a wave in E2M1) and leave as 1 KB stores: stored from the lanes, as words of 32-byte
+//   pieces, [10752, 2048] took 18 us and [10752, 6144] 41.
 //   Column axis: the amax over the lane's eight rows and the lanes l, l ^ 16, l ^ 32, l ^ 48 (two lane swaps); the codes
-//   are turned through LDS and leave in 16-byte chunks.
+//   are turned through LDS and leave in 16-byte chunks, 1 KB of whole 128-byte lines a wave.
 #include "abi_common.h"
 #include "mx4_device.h"
 
@@ -31,54 +33,84 @@ struct QuantArgs {
   int vec;  // rows are aligned to 16 bytes
 };
 
+__device__ __forceinline__ uint32_t word(const uint4& v, int p) { return p == 0 ? v.x : p == 1 ? v.y : p == 2 ? v.z : v.w; }
+
+// Column i of eight rows' groups (i a constant once unrolled)
+template <int kT>
+__device__ __forceinline__ Group<kT> column(const Group<kT>* v, int i) {
+  Group<kT> g;
+  uint32_t u[8];
+  if constexpr (kT == MXFP4_F32) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) u[k] = i < 4 ? word(v[k].w, i) : word(v[k].x, i - 4);
+    g.w = make_uint4(u[0], u[1], u[2], u[3]);
+    g.x = make_uint4(u[4], u[5], u[6], u[7]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)  // the low or the high halves of two rows' words
+      u[k] = __builtin_amdgcn_perm(word(v[2 * k + 1].w, i >> 1), word(v[2 * k].w, i >> 1), i & 1 ? 0x07060302u : 0x05040100u);
+    g.w = make_uint4(u[0], u[1], u[2], u[3]);
+  }
+  return g;
+}
+
 template <int kT, int kFmt, bool kRows, bool kCols>
 __global__ __launch_bounds__(kThreads) void quant_kernel(const QuantArgs a) {
   constexpr int kB = kFmt == MXFP4_E4M3 ? 8 : 4;         // bytes of eight codes
   constexpr int kLd = 16 * kB + 16;                      // row stride of the turned codes (128 codes and a pad)
+  constexpr int kWaveBytes = 32 * 16 * kB;               // codes of a wave's 32 rows
   __shared__ uint32_t stile[kTile], sttile[kCols ? kTile : 1];
   __shared__ __attribute__((aligned(16))) uint8_t qtt[kCols ? kTile * kLd : 16];
+  __shared__ __attribute__((aligned(16))) uint8_t qr[kRows ? 4 * kWaveBytes : 16];
   typedef typename Elem<kT>::T T;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, rg = lane >> 4, ch = lane & 15;
   const int64_t ct = blockIdx.x, rt = blockIdx.y;
-  const int64_t col = ct * kTile + ch * 8, row0 = rt * kTile + 32 * w + 8 * rg;
+  const int64_t col = ct * kTile + ch * 8, row32 = rt * kTile + 32 * w, row0 = row32 + 8 * rg;
   const T* x = reinterpret_cast<const T*>(a.x);
-  float v[8][8];
+  Group<kT> v[8];
   if (a.vec && (ct + 1) * kTile <= a.cols) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) load8<kT>(x + min(row0 + k, a.rows - 1) * a.ld + col, v[k]);
+    for (int k = 0; k < 8; ++k) v[k] = load_group<kT>(x + min(row0 + k, a.rows - 1) * a.ld + col);
   } else {
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const T t = x[min(row0 + k, a.rows - 1) * a.ld + min(col + i, a.cols - 1)];
-        v[k][i] = col + i < a.cols ? Elem<kT>::get(t) : 0.f;
-      }
+    for (int k = 0; k < 8; ++k) v[k] = load_group_edge<kT>(x + min(row0 + k, a.rows - 1) * a.ld, col, a.cols);
   }
   if (kCols) {  // rows past the end are zeros of the column axis
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[k][i] = row0 + k < a.rows ? v[k][i] : 0.f;
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t m = row0 + k < a.rows ? ~0u : 0u;
+      v[k].w = make_uint4(v[k].w.x & m, v[k].w.y & m, v[k].w.z & m, v[k].w.w & m);
+      if constexpr (kT == MXFP4_F32) v[k].x = make_uint4(v[k].x.x & m, v[k].x.y & m, v[k].x.z & m, v[k].x.w & m);
+    }
   }
   if (kRows) {
     uint8_t* sb = reinterpret_cast<uint8_t*>(stile);
+    uint8_t* mine = qr + w * kWaveBytes;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const uint32_t e = block_exponent<kFmt>(quad_umax(absmax8(v[k])));
+      const uint32_t e = block_exponent<kFmt>(quad_umax(v[k].absmax()));
       uint32_t c[2];
-      encode8<kFmt>(v[k], e, c);
-      const int64_t r = order_row(row0 + k, a.order);
-      if (row0 + k < a.rows) {
-        uint8_t* p = a.q + code_offset<kFmt>(r, col, a.q_tiles);
-        if constexpr (kFmt == MXFP4_E4M3) store_codes<true>(p, make_uint2(c[0], c[1]));
-        else store_codes<true>(p, c[0]);
-      }
+      encode_group<kT, kFmt>(v[k], e, c);
+      // the row's place among the wave's 32, which stay together in every order
+      const int rl = (int)order_row(8 * rg + k, a.order == MXFP4_ROWS_PLAIN ? MXFP4_ROWS_PLAIN : MXFP4_ROWS_PI);
+      uint8_t* p = mine + code_offset<kFmt>(rl, ch * 8, 1);
+      if constexpr (kFmt == MXFP4_E4M3) *reinterpret_cast<uint2*>(p) = make_uint2(c[0], c[1]);
+      else *reinterpret_cast<uint32_t*>(p) = c[0];
       // the gate and up orders spread a tile's rows over two scale tiles: their bytes go out one by one
       const uint8_t eb = row0 + k < a.rows ? (uint8_t)e : (uint8_t)0;
       if ((ch & 3) == 0) {
-        if (a.order < MXFP4_ROWS_GATE) sb[(r & 31) * 16 + w * 4 + (ch >> 2)] = eb;
-        else if (row0 + k < (a.rows + 31) / 32 * 32) a.s[blocked_offset(r, col >> 5, a.q_tiles)] = eb;
+        if (a.order < MXFP4_ROWS_GATE) sb[rl * 16 + w * 4 + (ch >> 2)] = eb;
+        else if (row0 + k < (a.rows + 31) / 32 * 32) a.s[blocked_offset(order_row(row0 + k, a.order), col >> 5, a.q_tiles)] = eb;
+      }
+    }
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // a wave reads back what it wrote itself
+    if (row32 < a.rows) {
+      const int64_t r = order_row(row32, a.order);  // the first row of the 32 in every order
+#pragma unroll
+      for (int j = 0; j < kWaveBytes / 1024; ++j) {
+        constexpr int kPer = kWaveBytes / 2048;  // KB of a 16-row block
+        store_codes<true>(a.q + ((r >> 4) + j / kPer) * a.q_tiles * (1024 * kPer) + (ct * kPer + j % kPer) * 1024 + lane * 16,
+                          *reinterpret_cast<const uint4*>(mine + j * 1024 + lane * 16));
       }
     }
   }
@@ -86,15 +118,13 @@ __global__ __launch_bounds__(kThreads) void quant_kernel(const QuantArgs a) {
     uint8_t* stb = reinterpret_cast<uint8_t*>(sttile);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      float t[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) t[k] = v[k][i];
-      uint32_t m = absmax8(t), pa, pb;
-      pair16(m, pa, pb);
+      const Group<kT> t = column<kT>(v, i);
+      uint32_t pa, pb;
+      pair16(t.absmax(), pa, pb);
       pair32(max(pa, pb), pa, pb);
       const uint32_t e = block_exponent<kFmt>(max(pa, pb));
       uint32_t c[2];
-      encode8<kFmt>(t, e, c);
+      encode_group<kT, kFmt>(t, e, c);
       const int cl = ch * 8 + i;  // column in the tile; its codes of rows 32 w + 8 rg ..
       // slots of eight codes, turned by the lane's column group so that a write instruction spreads over the banks
       const int slot = (4 * w + rg) ^ (ch & 12);
@@ -128,41 +158,74 @@ __global__ __launch_bounds__(kThreads) void quant_kernel(const QuantArgs a) {
                       reinterpret_cast<const uint4*>(sttile)[tid - 64]);
 }
 
-// Eight values a thread; odd widths end in a shorter piece.
+// A workgroup takes 16 rows of four column tiles; thread t row t / 16 and columns 8 (t % 16) .. of each.
 template <int kT, int kFmt>
 __global__ __launch_bounds__(kThreads) void dequant_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ s,
-                                                           int64_t rows, int64_t cols, int64_t tiles, int64_t per_row,
-                                                           void* out, int vec) {
-  const int64_t id = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  const int64_t r = id / per_row, c = (id - r * per_row) * 8;
-  if (r >= rows) return;
-  const uint32_t e = s[blocked_offset(r, c >> 5, tiles)];
-  const uint8_t* p = q + code_offset<kFmt>(r, c, tiles);
-  float v[8];
-  if constexpr (kFmt == MXFP4_E4M3) {
-    const uint2 w = *reinterpret_cast<const uint2*>(p);
+                                                           int64_t rows, int64_t cols, int64_t tiles, void* out, int vec) {
+  typedef typename Elem<kT>::T T;
+  const int64_t r = (int64_t)blockIdx.y * 16 + (threadIdx.x >> 4);
+  const int cl = (threadIdx.x & 15) * 8;
+  uint2 code[4];
+  uint32_t e[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t code = ((i < 4 ? w.x : w.y) >> (8 * (i & 3))) & 0xffu;
-      const uint32_t E = (code >> 3) & 15u, M = code & 7u;
-      float f = E == 0 ? (float)M * 0x1p-9f : __builtin_ldexpf((float)(8u + M), (int)E - 10);
-      f = (code & 0x80u) ? -f : f;
-      v[i] = (code & 0x7fu) == 0x7fu ? __uint_as_float(0x7fc00000u) : __builtin_ldexpf(f, (int)e - 127);
+  for (int j = 0; j < 4; ++j) {  // rows past the end lie in the operand's padding
+    const int64_t t = min((int64_t)blockIdx.x * 4 + j, tiles - 1);
+    const uint8_t* p = q + code_offset<kFmt>(r, t * 128 + cl, tiles);
+    if constexpr (kFmt == MXFP4_E4M3) code[j] = *reinterpret_cast<const uint2*>(p);
+    else code[j].x = *reinterpret_cast<const uint32_t*>(p);
+    e[j] = s[blocked_offset(r, t * 4 + (cl >> 5), tiles)];
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int64_t c = ((int64_t)blockIdx.x * 4 + j) * 128 + cl;
+    float v[8];
+    const uint32_t w[2] = {code[j].x, code[j].y};
+    // the hardware's conversion for scales whose products are normal numbers, else by hand (one branch a wave)
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(e[j] < 12u || e[j] > 245u) == 0, 1)) {
+      const float sc = __uint_as_float(e[j] << 23);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v2f f;
+        if constexpr (kFmt == MXFP4_E4M3) f = i & 1 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[i >> 1], sc, true)
+                                                    : __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[i >> 1], sc, false);
+        else f = i == 0   ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], sc, 0)
+                 : i == 1 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], sc, 1)
+                 : i == 2 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], sc, 2)
+                          : __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], sc, 3);
+        v[2 * i] = f[0];
+        v[2 * i + 1] = f[1];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float f;
+        bool nan = e[j] == 255u;
+        if constexpr (kFmt == MXFP4_E4M3) {
+          const uint32_t b = (w[i >> 2] >> (8 * (i & 3))) & 0xffu, E = (b >> 3) & 15u, M = b & 7u;
+          f = E == 0 ? (float)M * 0x1p-9f : __builtin_ldexpf((float)(8u + M), (int)E - 10);
+          f = b & 0x80u ? -f : f;
+          nan |= (b & 0x7fu) == 0x7fu;
+        } else {
+          const uint32_t b = (w[0] >> (4 * i)) & 15u, E = (b >> 1) & 3u, M = b & 1u;
+          f = E == 0 ? 0.5f * M : __builtin_ldexpf((float)(2u + M), (int)E - 2);
+          f = b & 8u ? -f : f;
+        }
+        v[i] = nan ? __uint_as_float(0x7fc00000u) : __builtin_ldexpf(f, (int)e[j] - 127);
+      }
     }
-  } else {
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t code = (w >> (4 * i)) & 15u, E = (code >> 1) & 3u, M = code & 1u;
-      const float f = E == 0 ? 0.5f * M : __builtin_ldexpf((float)(2u + M), (int)E - 2);
-      v[i] = __builtin_ldexpf((code & 8u) ? -f : f, (int)e - 127);
+    if (r < rows && c < cols) {
+      T* row = reinterpret_cast<T*>(out) + r * cols;
+      if (vec && c + 8 <= cols) {
+        if constexpr (kT == MXFP4_F32) store_run<kT, 8>(row, c, cols, true, v);
+        else
+          store_codes<true>(reinterpret_cast<uint8_t*>(row + c),
+                            make_uint4(round2<kT>(v[0], v[1]), round2<kT>(v[2], v[3]), round2<kT>(v[4], v[5]),
+                                       round2<kT>(v[6], v[7])));
+      } else {
+        store_run<kT, 8>(row, c, cols, false, v);
+      }
     }
   }
-  if (e == 255u) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(0x7fc00000u);
-  }
-  store_run<kT, 8>(reinterpret_cast<typename Elem<kT>::T*>(out) + r * cols, c, cols, vec, v);
 }
 
 template <int kT, int kFmt>
@@ -174,14 +237,15 @@ void launch_quant(const QuantArgs& a, dim3 grid, hipStream_t st) {
 
 template <int kT>
 void launch_dequant(const void* q, const void* s, int64_t rows, int64_t cols, int64_t fmt, void* out, int vec,
-                    int64_t per_row, unsigned blocks, hipStream_t st) {
+                    hipStream_t st) {
   const int64_t tiles = (cols + 127) / 128;
+  const dim3 grid((unsigned)((tiles + 3) / 4), (unsigned)((rows + 15) / 16));
   if (fmt == MXFP4_E4M3)
-    dequant_kernel<kT, MXFP4_E4M3><<<blocks, kThreads, 0, st>>>((const uint8_t*)q, (const uint8_t*)s, rows, cols, tiles,
-                                                                per_row, out, vec);
+    dequant_kernel<kT, MXFP4_E4M3><<<grid, kThreads, 0, st>>>((const uint8_t*)q, (const uint8_t*)s, rows, cols, tiles, out,
+                                                              vec);
   else
-    dequant_kernel<kT, MXFP4_E2M1><<<blocks, kThreads, 0, st>>>((const uint8_t*)q, (const uint8_t*)s, rows, cols, tiles,
-                                                                per_row, out, vec);
+    dequant_kernel<kT, MXFP4_E2M1><<<grid, kThreads, 0, st>>>((const uint8_t*)q, (const uint8_t*)s, rows, cols, tiles, out,
+                                                              vec);
 }
 
 int elem_size(int64_t type) { return type == MXFP4_F32 ? 4 : 2; }
@@ -231,13 +295,12 @@ extern "C" int mxfp4_dequant(const void* q, const void* s, int64_t rows, int64_t
   MX_CHECK_ARG(q && s && out, "mxfp4_dequant: null pointer");
   MX_CHECK_ARG(mx_aligned(q, 16) && mx_aligned(s, 16) && mx_aligned(out, elem_size(type)),
                "mxfp4_dequant: misaligned buffer");
-  const int64_t per_row = (cols + 7) / 8, blocks = (rows * per_row + kThreads - 1) / kThreads;
-  MX_CHECK_ARG(blocks <= 0x7fffffff, "mxfp4_dequant: too large");
+  MX_CHECK_ARG((rows + 15) / 16 <= 65535 && cols < (1LL << 36), "mxfp4_dequant: too large");
   const int vec = mx_aligned(out, 16) && cols * elem_size(type) % 16 == 0;
   const hipStream_t hs = (hipStream_t)stream;
-  if (type == MXFP4_BF16) launch_dequant<MXFP4_BF16>(q, s, rows, cols, fmt, out, vec, per_row, (unsigned)blocks, hs);
-  else if (type == MXFP4_F16) launch_dequant<MXFP4_F16>(q, s, rows, cols, fmt, out, vec, per_row, (unsigned)blocks, hs);
-  else launch_dequant<MXFP4_F32>(q, s, rows, cols, fmt, out, vec, per_row, (unsigned)blocks, hs);
+  if (type == MXFP4_BF16) launch_dequant<MXFP4_BF16>(q, s, rows, cols, fmt, out, vec, hs);
+  else if (type == MXFP4_F16) launch_dequant<MXFP4_F16>(q, s, rows, cols, fmt, out, vec, hs);
+  else launch_dequant<MXFP4_F32>(q, s, rows, cols, fmt, out, vec, hs);
   MX_CHECK_LAUNCH("mxfp4_dequant");
   return MXFP8_OK;
 }
