@@ -7,8 +7,12 @@
 // tokens as the other operand's rows; rows past M repeat the last one.  Its operand of x needs no exchange in E2M1 (lane l
 // holds a whole 32-block of token l % 16) and two lane swaps in E4M3 (each block lies in two lanes), so every wave
 // quantizes what it multiplies, from registers, while its weight blocks are under way.
+//
+// thin_kernel does the same for 17 to 64 rows of a quantized operand, which lies in memory as the instruction takes it: up to
+// four 16-row blocks of tokens for each weight block.  Tiles of 64 rows leave most CUs without work there.
 #include "abi_common.h"
 #include "mx4_device.h"
+#include "mx4_plan.h"
 
 using namespace mx4;
 
@@ -27,6 +31,7 @@ struct FewArgs {
   const void* add;
   int64_t ld_add;
   int fn, vec_x, vec_c;
+  const uint8_t* sx;
 };
 
 // 16 values of columns k.. of a row, zeros past K
@@ -74,6 +79,52 @@ __device__ __forceinline__ v8i operand(const Group<kT>* w, int g, uint32_t& scal
   return r;
 }
 
+// The weight rows of a workgroup: 16-row block `blk` of B, or half blk % 2 of gate block and up block blk / 2
+template <bool kGated>
+struct Rows {
+  static constexpr int kB = kGated ? 2 : 1;
+  const uint8_t* w[kB];  // this lane's 16 bytes and scale byte of K tile 0
+  const uint8_t* s[kB];
+  __device__ __forceinline__ Rows(const uint8_t* b, const uint8_t* sb, int64_t blk, int64_t kt, int r16, int g) {
+#pragma unroll
+    for (int i = 0; i < kB; ++i) {
+      const int64_t rb = kGated ? (blk >> 1) * 64 + (blk & 1) * 16 + 32 * i : blk * 16, r = rb + r16;
+      w[i] = b + (rb >> 4) * kt * 1024 + (g >> 1) * 512 + r16 * 32 + (((g & 1) ^ (r16 >> 3)) << 4);
+      s[i] = sb + (r >> 7) * kt * 512 + (r & 31) * 16 + ((r & 127) >> 5) * 4 + g;
+    }
+  }
+};
+__device__ __forceinline__ v8i operand4(uint4 v) { return v8i{(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0}; }
+template <int kFmt>
+__device__ __forceinline__ v4f mma(v8i w, uint32_t ws, v8i x, uint32_t xs, v4f acc) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, acc, 4, kFmt == MXFP4_E4M3 ? 0 : 4, 0, (int)ws, 0, (int)xs);
+}
+
+// Sums of a 16 x 16 block (gate and up): lane l holds token l % 16 and, of weight rows 4 (l / 16) + 0..3 of the 16, four
+// consecutive columns (the PI order)
+template <int kT, bool kGated>
+__device__ __forceinline__ void finish(const FewArgs& a, int64_t blk, int lane, int m, const f32x4* s) {
+  typedef typename Elem<kT>::T T;
+  const int g = lane >> 4;
+  const int64_t c = (blk >> 1) * 32 + (g & 1) * 16 + (2 * (int)(blk & 1) + (g >> 1)) * 4;
+  if (m >= a.M) return;
+  float v[4], u[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    v[q] = s[0][q];
+    if constexpr (kGated) {
+      u[q] = s[1][q];
+      if (a.add && c + q < a.N) {
+        const T* ad = reinterpret_cast<const T*>(a.add) + m * a.ld_add;
+        v[q] += Elem<kT>::get(ad[c + q]);
+        u[q] += Elem<kT>::get(ad[a.N + c + q]);
+      }
+      v[q] = (a.fn == MXFP4_SILU ? gate_fn<MXFP4_SILU>(v[q]) : gate_fn<MXFP4_GELU>(v[q])) * u[q];
+    }
+  }
+  store_run<kT, 4>(reinterpret_cast<T*>(a.c) + m * a.ldc, c, a.N, a.vec_c, v);
+}
+
 template <int kT, int kFmt, bool kGated, int kWaves>
 __global__ __launch_bounds__(64 * kWaves) void few_kernel(const FewArgs a) {
   typedef typename Elem<kT>::T T;
@@ -81,24 +132,8 @@ __global__ __launch_bounds__(64 * kWaves) void few_kernel(const FewArgs a) {
   __shared__ __attribute__((aligned(16))) f32x4 part[kWaves][kB][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r16 = lane & 15, g = lane >> 4;
-  // the weight rows: 16-row block `blockIdx.x` of B, or half h of gate block and up block j
-  const int64_t blk = blockIdx.x;
-  int64_t rb[kB];  // first row of the 16
-  if constexpr (kGated) {
-    rb[0] = (blk >> 1) * 64 + (blk & 1) * 16;
-    rb[1] = rb[0] + 32;
-  } else {
-    rb[0] = blk * 16;
-  }
+  const Rows<kGated> rows(a.b, a.sb, blockIdx.x, a.kt, r16, g);
   const int per = (a.kt + kWaves - 1) / kWaves, t0 = wave * per, t1 = min(a.kt, t0 + per);
-  const uint8_t* wp[kB];
-  const uint8_t* sp[kB];
-#pragma unroll
-  for (int i = 0; i < kB; ++i) {
-    wp[i] = a.b + (rb[i] >> 4) * a.kt * 1024 + (g >> 1) * 512 + r16 * 32 + (((g & 1) ^ (r16 >> 3)) << 4);
-    const int64_t r = rb[i] + r16;
-    sp[i] = a.sb + (r >> 7) * a.kt * 512 + (r & 31) * 16 + ((r & 127) >> 5) * 4 + g;
-  }
   const T* xrow = reinterpret_cast<const T*>(a.x) + (int64_t)min(r16, a.M - 1) * a.ld_x;
   const int k0 = kFmt == MXFP4_E4M3 ? 16 * g : 32 * g, k1 = kFmt == MXFP4_E4M3 ? 64 + 16 * g : 32 * g + 16;
   v4f acc[kB];
@@ -113,8 +148,8 @@ __global__ __launch_bounds__(64 * kWaves) void few_kernel(const FewArgs a) {
       const int64_t tu = min(t + u, t1 - 1);
 #pragma unroll
       for (int i = 0; i < kB; ++i) {
-        wv[u][i] = *reinterpret_cast<const uint4*>(wp[i] + tu * 1024);
-        ws[u][i] = sp[i][tu * 512];
+        wv[u][i] = *reinterpret_cast<const uint4*>(rows.w[i] + tu * 1024);
+        ws[u][i] = rows.s[i][tu * 512];
       }
     }
 #pragma unroll
@@ -129,43 +164,95 @@ __global__ __launch_bounds__(64 * kWaves) void few_kernel(const FewArgs a) {
       uint32_t xs;
       const v8i xo = operand<kT, kFmt>(xv[u], g, xs);
 #pragma unroll
-      for (int i = 0; i < kB; ++i) {
-        const v8i wo = {(int)wv[u][i].x, (int)wv[u][i].y, (int)wv[u][i].z, (int)wv[u][i].w, 0, 0, 0, 0};
-        acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wo, xo, acc[i], 4, kFmt == MXFP4_E4M3 ? 0 : 4, 0,
-                                                                  (int)ws[u][i], 0, (int)xs);
-      }
+      for (int i = 0; i < kB; ++i) acc[i] = mma<kFmt>(operand4(wv[u][i]), ws[u][i], xo, xs, acc[i]);
     }
   }
 #pragma unroll
   for (int i = 0; i < kB; ++i) part[wave][i][lane] = f32x4{acc[i][0], acc[i][1], acc[i][2], acc[i][3]};
   __syncthreads();
   if (wave) return;
-  float v[kB][4];
+  f32x4 s[kB];
 #pragma unroll
   for (int i = 0; i < kB; ++i) {
-    f32x4 s = part[0][i][lane];
+    s[i] = part[0][i][lane];
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) s += part[w][i][lane];
-#pragma unroll
-    for (int q = 0; q < 4; ++q) v[i][q] = s[q];
+    for (int w = 1; w < kWaves; ++w) s[i] += part[w][i][lane];
   }
-  // lane: token r16, weight rows 4 g + 0..3 of the 16, which are 4 consecutive columns (the PI order)
-  const int half = (int)(blk & 1);
-  const int64_t c = (blk >> 1) * 32 + (g & 1) * 16 + (2 * half + (g >> 1)) * 4;
-  if (r16 >= a.M) return;
-  T* out = reinterpret_cast<T*>(a.c) + r16 * a.ldc;
-  if constexpr (kGated) {
+  finish<kT, kGated>(a, blockIdx.x, lane, r16, s);
+}
+
+// kTB blocks of 16 rows of a quantized operand (a.x its codes, a.sx its scales)
+template <int kT, int kFmt, bool kGated, int kTB>
+__global__ __launch_bounds__(512) void thin_kernel(const FewArgs a) {
+  constexpr int kB = kGated ? 2 : 1, kWaves = 8, kU = 2, kA = kFmt == MXFP4_E4M3 ? 2 : 1;
+  __shared__ __attribute__((aligned(16))) f32x4 part[kWaves][kB][kTB][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r16 = lane & 15, g = lane >> 4;
+  const Rows<kGated> rows(a.b, a.sb, blockIdx.x, a.kt, r16, g);
+  const uint8_t* xp[kTB];
+  const uint8_t* xsp[kTB];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      if (a.add && c + q < a.N) {
-        const T* ad = reinterpret_cast<const T*>(a.add) + r16 * a.ld_add;
-        v[0][q] += Elem<kT>::get(ad[c + q]);
-        v[1][q] += Elem<kT>::get(ad[a.N + c + q]);
+  for (int b = 0; b < kTB; ++b) {  // blocks past the rows re-read the last one and are not stored
+    const int blk = min(b, (a.M - 1) >> 4), r = blk * 16 + r16;
+    xp[b] = reinterpret_cast<const uint8_t*>(a.x) + (int64_t)blk * a.kt * (1024 * kA) +
+            (kA == 2 ? r16 * 64 + ((g ^ (r16 >> 2)) << 4) : (g >> 1) * 512 + r16 * 32 + (((g & 1) ^ (r16 >> 3)) << 4));
+    xsp[b] = a.sx + (r & 31) * 16 + (r >> 5) * 4 + g;
+  }
+  v4f acc[kB][kTB];
+#pragma unroll
+  for (int i = 0; i < kB; ++i)
+#pragma unroll
+    for (int b = 0; b < kTB; ++b) acc[i][b] = v4f{0.f, 0.f, 0.f, 0.f};
+  const int per = (a.kt + kWaves - 1) / kWaves, t0 = wave * per, t1 = min(a.kt, t0 + per);
+  for (int t = t0; t < t1; t += kU) {
+    uint4 wv[kU][kB], xv[kU][kTB][kA];
+    uint32_t ws[kU][kB], xs[kU][kTB];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const int64_t tu = min(t + u, t1 - 1);
+#pragma unroll
+      for (int i = 0; i < kB; ++i) {
+        wv[u][i] = *reinterpret_cast<const uint4*>(rows.w[i] + tu * 1024);
+        ws[u][i] = rows.s[i][tu * 512];
       }
-      v[0][q] = (a.fn == MXFP4_SILU ? gate_fn<MXFP4_SILU>(v[0][q]) : gate_fn<MXFP4_GELU>(v[0][q])) * v[1][q];
+#pragma unroll
+      for (int b = 0; b < kTB; ++b) {
+#pragma unroll
+        for (int h = 0; h < kA; ++h) xv[u][b][h] = *reinterpret_cast<const uint4*>(xp[b] + (tu * kA + h) * 1024);
+        xs[u][b] = xsp[b][tu * 512];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      if (t + u >= t1) break;
+#pragma unroll
+      for (int b = 0; b < kTB; ++b) {
+        v8i x = operand4(xv[u][b][0]);
+        if constexpr (kA == 2) {
+          x[4] = (int)xv[u][b][1].x;
+          x[5] = (int)xv[u][b][1].y;
+          x[6] = (int)xv[u][b][1].z;
+          x[7] = (int)xv[u][b][1].w;
+        }
+#pragma unroll
+        for (int i = 0; i < kB; ++i) acc[i][b] = mma<kFmt>(operand4(wv[u][i]), ws[u][i], x, xs[u][b], acc[i][b]);
+      }
     }
   }
-  store_run<kT, 4>(out, c, a.N, a.vec_c, v[0]);
+#pragma unroll
+  for (int i = 0; i < kB; ++i)
+#pragma unroll
+    for (int b = 0; b < kTB; ++b) part[wave][i][b][lane] = f32x4{acc[i][b][0], acc[i][b][1], acc[i][b][2], acc[i][b][3]};
+  __syncthreads();
+  if (wave >= kTB) return;
+  f32x4 s[kB];
+#pragma unroll
+  for (int i = 0; i < kB; ++i) {
+    s[i] = part[0][i][wave][lane];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) s[i] += part[w][i][wave][lane];
+  }
+  finish<kT, kGated>(a, blockIdx.x, lane, wave * 16 + r16, s);
 }
 
 template <int kT, int kFmt, bool kGated>
@@ -189,6 +276,21 @@ int run(FewArgs& a, int64_t fmt, int64_t type, const char* what, hipStream_t st)
   return MXFP8_OK;
 }
 
+template <int kT, int kFmt, bool kGated>
+void launch_thin(const FewArgs& a, unsigned blocks, hipStream_t st) {
+  if (a.M <= 32) thin_kernel<kT, kFmt, kGated, 2><<<blocks, 512, 0, st>>>(a);
+  else thin_kernel<kT, kFmt, kGated, 4><<<blocks, 512, 0, st>>>(a);
+}
+template <bool kGated>
+void run_thin(const FewArgs& a, int64_t fmt, int64_t type, hipStream_t st) {
+  const unsigned blocks = (unsigned)(((int64_t)a.N + 31) / 32 * 2);
+  const bool f8 = fmt == MXFP4_E4M3;
+  if (type == MXFP4_BF16)
+    f8 ? launch_thin<MXFP4_BF16, MXFP4_E4M3, kGated>(a, blocks, st) : launch_thin<MXFP4_BF16, MXFP4_E2M1, kGated>(a, blocks, st);
+  else
+    f8 ? launch_thin<MXFP4_F16, MXFP4_E4M3, kGated>(a, blocks, st) : launch_thin<MXFP4_F16, MXFP4_E2M1, kGated>(a, blocks, st);
+}
+
 int check(const char* what, const void* x, int64_t ld_x, int64_t fmt, const void* b, const void* sb, int64_t M, int64_t N,
           int64_t K, const void* c, int64_t ldc, int64_t type) {
   MX_CHECK_ARG(M >= 0 && M <= MXFP4_FEW_ROWS && N > 0 && N < (1LL << 29) && K > 0 && K < (1LL << 26),
@@ -205,11 +307,19 @@ int check(const char* what, const void* x, int64_t ld_x, int64_t fmt, const void
 
 }  // namespace
 
+// mx4_gemm.hip's call for kMx4ThinRows rows at most (mx4_plan.h), its arguments checked there
+void mx4_thin(bool gated, const void* q, const void* sq, int64_t fmt, const void* b, const void* sb, int M, int N, int kt,
+              const void* add, int64_t ld_add, int fn, void* c, int64_t ldc, int64_t type, hipStream_t st) {
+  const FewArgs a{q, 0, (const uint8_t*)b, (const uint8_t*)sb, M, N, kt * 128, kt, c, ldc, add, ld_add, fn, 0,
+                  mx_aligned(c, 8) && ldc % 4 == 0, (const uint8_t*)sq};
+  gated ? run_thin<true>(a, fmt, type, st) : run_thin<false>(a, fmt, type, st);
+}
+
 extern "C" int mxfp4_few(const void* x, int64_t ld_x, int64_t fmt, const void* b, const void* sb, int64_t M, int64_t N,
                          int64_t K, void* c, int64_t ldc, int64_t type, void* stream) {
   if (int rc = check("mxfp4_few", x, ld_x, fmt, b, sb, M, N, K, c, ldc, type)) return rc;
   if (M == 0) return MXFP8_OK;
-  FewArgs a{x, ld_x, (const uint8_t*)b, (const uint8_t*)sb, (int)M, (int)N, (int)K, 0, c, ldc, nullptr, 0, 0, 0, 0};
+  FewArgs a{x, ld_x, (const uint8_t*)b, (const uint8_t*)sb, (int)M, (int)N, (int)K, 0, c, ldc, nullptr, 0, 0, 0, 0, nullptr};
   return run<false>(a, fmt, type, "mxfp4_few", (hipStream_t)stream);
 }
 
@@ -220,6 +330,6 @@ extern "C" int mxfp4_few_gated(const void* x, int64_t ld_x, int64_t fmt, const v
   MX_CHECK_ARG(fn == MXFP4_SILU || fn == MXFP4_GELU, "mxfp4_few_gated: unknown gate function %lld", (long long)fn);
   MX_CHECK_ARG(!add || ((ld_add == 0 || ld_add >= 2 * N) && mx_aligned(add, 2)), "mxfp4_few_gated: bad addend");
   if (M == 0) return MXFP8_OK;
-  FewArgs a{x, ld_x, (const uint8_t*)b, (const uint8_t*)sb, (int)M, (int)N, (int)K, 0, h, ldh, add, ld_add, (int)fn, 0, 0};
+  FewArgs a{x, ld_x, (const uint8_t*)b, (const uint8_t*)sb, (int)M, (int)N, (int)K, 0, h, ldh, add, ld_add, (int)fn, 0, 0, nullptr};
   return run<true>(a, fmt, type, "mxfp4_few_gated", (hipStream_t)stream);
 }

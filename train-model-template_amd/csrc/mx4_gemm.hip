@@ -14,8 +14,12 @@
 
 #include "abi_common.h"
 #include "mx4_device.h"
+#include "mx4_plan.h"
 
 using namespace mx4;
+
+void mx4_thin(bool gated, const void* q, const void* sq, int64_t fmt, const void* b, const void* sb, int M, int N, int kt,
+              const void* add, int64_t ld_add, int fn, void* c, int64_t ldc, int64_t type, hipStream_t st);  // mx4_few.hip
 
 namespace {
 
@@ -36,7 +40,7 @@ struct Shape {
   static constexpr int kPieces = (kTilesA + kTilesB) * 2, kSS = (kPieces + kWaves - 1) / kWaves;
   static constexpr int kDma = kSA + kSB + kSS;
   static constexpr int kRing = kStages * kStageBytes;
-  static_assert(kSA * kWaves * 1024 == kBytesA && kSB * kWaves * 1024 == kBytesB && kRing <= 160 * 1024, "shape");
+  static_assert(kSA * kWaves * 1024 == kBytesA && kSB * kWaves * 1024 == kBytesB && kRing <= 80 * 1024, "shape");
 };
 
 struct GemmArgs {
@@ -58,12 +62,12 @@ struct GemmArgs {
 
 enum Epi { kPlain, kGated };
 
+// The tile of this workgroup.  Workgroup i runs on XCD i % 8; each XCD takes a contiguous range of tiles in groups of 1024
+// rows, M fastest, so that the tiles of an XCD share panels of A and B in its L2.
 template <class S>
 __device__ __forceinline__ bool tile_of(const GemmArgs& g, int& mt, int& nt) {
-  // workgroup i runs on XCD i % 8, each XCD takes a contiguous range of tiles in groups of 1024 rows, M fastest, so
-  // that the tiles of an XCD share panels of A and B in its L2
-  const int t = (blockIdx.x & 7) * g.per + (blockIdx.x >> 3);
-  if ((int)(blockIdx.x >> 3) >= g.per || t >= g.tm * g.tn) return false;
+  const int j = blockIdx.x >> 3, t = (blockIdx.x & 7) * g.per + j;
+  if (j >= g.per || t >= g.tm * g.tn) return false;
   const int grp = t / (S::kGroupM * g.tn), r = t - grp * (S::kGroupM * g.tn);
   const int rows = min(S::kGroupM, g.tm - grp * S::kGroupM);
   mt = grp * S::kGroupM + r % rows;
@@ -186,7 +190,7 @@ __device__ __forceinline__ void store_gated(const GemmArgs& g, int m0, int n0, i
 
 // ---- the kernel
 template <class S, int kEpi>
-__global__ __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_eu(S::kWaves * S::kMB * S::kNB >= 64 && S::kWaves == 4 ? 1 : 2)))
+__global__ __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_eu(2)))
 void gemm_kernel(const GemmArgs g) {
   constexpr int kMB = S::kMB, kNB = S::kNB;
   __shared__ __attribute__((aligned(16))) uint8_t lds[S::kRing];
@@ -233,7 +237,7 @@ void gemm_kernel(const GemmArgs g) {
     so[j] = S::kOffS + pc * 256;
   }
   const uint32_t lds0 = lds_addr(lds);
-  const int last = (S::kKS == 2 ? kt : 2 * kt) - 1;
+  const int last = (S::kKS == 2 ? kt : 2 * kt) - 1;  // stage
   auto dma = [&](int s, int slot, int d) {  // DMA d of stage s into ring slot `slot`
     const uint32_t st = lds0 + slot * S::kStageBytes;
     if (d < S::kSA)
@@ -387,14 +391,15 @@ void gemm_kernel(const GemmArgs g) {
   }
 }
 
+// Every ring leaves room for two workgroups a CU, so that one's pipeline fill, barriers and epilogue overlap the other's
+// products: 256 x 256 tiles with one took 87 us (E2M1, 10752 x 6144 x 2048) and 148 (10752 x 2048 x 12288) where these take 78
+// and 128.  In Tall the E4M3 stages are 64 codes wide, the E2M1 ones 128 (half the barriers).
 template <int kAF>
-using Big = Shape<kAF, 2, 4, 4, 2, 2, kAF == MXFP4_E4M3 ? 3 : 4>;  // 256 x 256, 8 waves, one workgroup a CU
+using Tall = Shape<kAF, 2, 4, 4, 1, kAF == MXFP4_E4M3 ? 1 : 2, 3>;  // 256 x 128, 65 or 76 KB
 template <int kAF>
-using Tall = Shape<kAF, 2, 4, 4, 1, kAF == MXFP4_E4M3 ? 1 : 2, 3>;  // 256 x 128, 4 waves, two a CU
+using Mid = Shape<kAF, 2, 2, 2, 2, 2, kAF == MXFP4_E4M3 ? 3 : 4>;  // 128 x 128, 75 or 68 KB
 template <int kAF>
-using Mid = Shape<kAF, 2, 2, 2, 2, 2, kAF == MXFP4_E4M3 ? 3 : 4>;  // 128 x 128, 4 waves, two a CU
-template <int kAF>
-using Low = Shape<kAF, 1, 2, 2, 2, 2, 4>;  // 64 x 128, 4 waves, two (three) a CU
+using Low = Shape<kAF, 1, 2, 2, 2, 2, 4>;  // 64 x 128, 68 or 52 KB
 
 template <class S, int kEpi>
 int launch(GemmArgs& g, const char* what, hipStream_t st) {
@@ -411,19 +416,15 @@ int launch(GemmArgs& g, const char* what, hipStream_t st) {
 
 template <int kEpi, int kAF>
 int dispatch(GemmArgs& g, const char* what, hipStream_t st) {
-  const int64_t big = ((int64_t)g.M + 255) / 256 * ((g.rows_b + 255) / 256);
-  const int64_t mid = ((int64_t)g.M + 127) / 128 * ((g.rows_b + 127) / 128);
-  if (const char* e = getenv("MX4_SHAPE")) {
-    switch (atoi(e)) {
-      case 0: return launch<Big<kAF>, kEpi>(g, what, st);
-      case 1: return launch<Tall<kAF>, kEpi>(g, what, st);
-      case 2: return launch<Mid<kAF>, kEpi>(g, what, st);
-      case 3: return launch<Low<kAF>, kEpi>(g, what, st);
-    }
+  switch (mx4_shape(g.M, g.rows_b, g.kt, kAF == MXFP4_E4M3, g.b_pi && g.type != MXFP4_F32 && !g.gu, 256)) {
+    case kMx4Thin:
+      mx4_thin(kEpi == kGated, g.a, g.sa, kAF, g.b, g.sb, g.M, g.N, g.kt, g.add, g.ld_add, g.fn, g.c, g.ldc, g.type, st);
+      MX_CHECK_LAUNCH(what);
+      return MXFP8_OK;
+    case kMx4Tall: return launch<Tall<kAF>, kEpi>(g, what, st);
+    case kMx4Mid: return launch<Mid<kAF>, kEpi>(g, what, st);
+    default: return launch<Low<kAF>, kEpi>(g, what, st);
   }
-  if (big >= 200) return launch<Big<kAF>, kEpi>(g, what, st);
-  if (mid >= 256) return launch<Mid<kAF>, kEpi>(g, what, st);
-  return launch<Low<kAF>, kEpi>(g, what, st);
 }
 template <int kEpi>
 int dispatch(GemmArgs& g, int64_t a_fmt, const char* what, hipStream_t st) {
