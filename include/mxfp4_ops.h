@@ -101,7 +101,7 @@ int mxfp4_few_gated(const void* x, int64_t ld_x, int64_t fmt, const void* b, con
 #define DISTILL_FINISH 2
 #define DISTILL_MAX_K 1024
 #define DISTILL_MAX_PARTS 256
-int64_t distill_parts(int64_t T, int64_t V);
+int64_t distill_parts(int64_t T, int64_t V, int64_t type);
 int64_t distill_workspace_size(int64_t T, int64_t k, int64_t parts);
 int distill_topk_kl(const void* logits, int64_t type, int64_t ld, int64_t T, int64_t V, const void* idx, int64_t idx_bytes,
                     int64_t ld_idx, const float* t, int64_t ld_t, int64_t k, float tau, const float* lse,

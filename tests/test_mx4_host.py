@@ -110,7 +110,7 @@ def test_refusals(lib):
 
 def test_plans(lib):
     assert lib.mxfp4_gated_saved_elems(I(33), I(65)) == 2 * 3 * 2048
-    parts = lambda T, V: lib.distill_parts(I(T), I(V))  # noqa: E731
+    parts = lambda T, V: lib.distill_parts(I(T), I(V), I(0))  # noqa: E731
     assert parts(4096, 65536) == 1 and parts(1, 1000) == 1 and parts(1, 65536) > 1
     for T in (1, 7, 300, 5000):
         for V in (1, 1000, 248001, 1 << 22):

@@ -54,31 +54,51 @@ __device__ __forceinline__ Sum join(Sum a, Sum b, float c) {
   const float m = fmaxf(a.m, b.m);
   return Sum{m, a.s * __builtin_amdgcn_exp2f((a.m - m) * c) + b.s * __builtin_amdgcn_exp2f((b.m - m) * c)};
 }
+// f over the 64 lanes, in every lane: lane swaps in the VALU (quad permutations, mirrors of 8 and of 16 lanes, swaps of 16 and
+// of 32), where shuffles go through LDS
+template <int kDpp>
+__device__ __forceinline__ float dpp(float v) {
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), kDpp, 0xF, 0xF, true));
+}
+__device__ __forceinline__ float first_lane(float v) {
+  return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v)));
+}
 template <class F>
 __device__ __forceinline__ float wave_reduce(float v, F f) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) v = f(v, __shfl_xor(v, o));
-  return v;
+  v = f(v, dpp<0xB1>(v));   // lane ^ 1
+  v = f(v, dpp<0x4E>(v));   // lane ^ 2
+  v = f(v, dpp<0x141>(v));  // 7 - lane of 8
+  v = f(v, dpp<0x140>(v));  // 15 - lane of 16
+  uint32_t a, b;
+  pair16(__float_as_uint(v), a, b);
+  v = f(__uint_as_float(a), __uint_as_float(b));
+  pair32(__float_as_uint(v), a, b);
+  return f(__uint_as_float(a), __uint_as_float(b));
 }
 __device__ __forceinline__ float wave_sum(float v) {
   return wave_reduce(v, [](float a, float b) { return a + b; });
 }
 __device__ __forceinline__ float wave_max(float v) {  // NaN stays
-  return wave_reduce(v, [](float a, float b) { return (a > b || a != a) ? a : b; });
+  return wave_reduce(v, [](float a, float b) { return a > b || a != a ? a : b; });
+}
+// The sum of all lanes: against the wave's maximum each lane is scaled once
+__device__ __forceinline__ Sum wave_join(Sum a, float c) {
+  const float m = wave_reduce(a.m, [](float x, float y) { return fmaxf(x, y); });
+  return Sum{m, wave_sum(a.s * __builtin_amdgcn_exp2f((a.m - m) * c))};
 }
 template <int kWaves>
 __device__ __forceinline__ Sum block_join(Sum a, float c, float* sh) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) a = join(a, Sum{__shfl_xor(a.m, o), __shfl_xor(a.s, o)}, c);
-  if ((threadIdx.x & 63) == 0) {
+  a = wave_join(a, c);
+  const int lane = threadIdx.x & 63;
+  if (lane == 0) {
     sh[threadIdx.x >> 6] = a.m;
     sh[kWaves + (threadIdx.x >> 6)] = a.s;
   }
   __syncthreads();
-  Sum r{sh[0], sh[kWaves]};
-#pragma unroll
-  for (int w = 1; w < kWaves; ++w) r = join(r, Sum{sh[w], sh[kWaves + w]}, c);
-  return r;
+  const int w = lane & (kWaves - 1);  // kWaves is a power of two: every wave's sum 64 / kWaves times
+  const Sum r = wave_join(Sum{sh[w], sh[kWaves + w]}, c);
+  // one lane's: the others may have added with a product kept unrounded (a fused multiply-add), an ulp apart
+  return Sum{first_lane(r.m), first_lane(r.s) * ((float)kWaves / 64.f)};
 }
 
 template <int kT>
@@ -380,10 +400,18 @@ void launch(const Args& a0, int64_t T, int stages, hipStream_t st) {
 
 }  // namespace
 
-extern "C" int64_t distill_parts(int64_t T, int64_t V) {
+// Splitting costs a launch and a second reading of the row, and pays where few long rows leave most CUs idle.  us with the
+// gradient, whole / split: 16 rows of 128 KB 12.2 / 9.4 (16 pieces), of 496 KB 32 / 12.6; one row of 496 KB 31 / 10.2 (32);
+// 64 rows of 128 KB 15.7 / 15.0, of 256 KB 20.0 / 13.4 (8), of 1 MB 46 / 37; 128 rows of 256 KB 24.3 / 22.2, of 1 MB 60 / 64;
+// 16 rows of 32 KB 10.7 / 12.4.
+extern "C" int64_t distill_parts(int64_t T, int64_t V, int64_t type) {
   if (T <= 0 || V <= 0) return 1;
-  const int64_t parts = std::max(std::min((int64_t)512 / T, V / 8192), (V + kMaxPiece - 1) / kMaxPiece);
-  return std::min<int64_t>(std::max<int64_t>(parts, 1), DISTILL_MAX_PARTS);
+  const int64_t bytes = V * (type == MXFP4_F32 ? 4 : 2);
+  int64_t parts = 1;
+  if (T <= 64 && bytes >= (T <= 16 ? 96 << 10 : 192 << 10))
+    parts = std::min<int64_t>({32, std::max<int64_t>(256 / T, 8), bytes >> 13});  // pieces of 8 KB at least
+  parts = std::max(parts, (V + kMaxPiece - 1) / kMaxPiece);
+  return std::min<int64_t>(parts, DISTILL_MAX_PARTS);
 }
 
 extern "C" int64_t distill_workspace_size(int64_t T, int64_t k, int64_t parts) {

@@ -400,7 +400,7 @@ Kl kl_call(const Tensor& z, const Tensor& idx, const Tensor& t, double tau, cons
     need(lse->dim() == 1 && lse->size(0) == T, what, "one teacher logsumexp a row");
     c.lse = lse->to(at::kFloat).contiguous();
   }
-  c.parts = distill_parts(T, V);
+  c.parts = distill_parts(T, V, type_of(z, what));
   return c;
 }
 

@@ -68,9 +68,15 @@ __global__ __launch_bounds__(kThreads) void quant_kernel(const QuantArgs a) {
   const int64_t col = ct * kTile + ch * 8, row32 = rt * kTile + 32 * w, row0 = row32 + 8 * rg;
   const T* x = reinterpret_cast<const T*>(a.x);
   Group<kT> v[8];
-  if (a.vec && (ct + 1) * kTile <= a.cols) {
+  if (a.vec && ((ct + 1) * kTile <= a.cols || a.cols % 8 == 0)) {
+    // a row's last tile ends with a whole group: lanes past it read the group before and take zeros
+    const int64_t cl = min(col, a.cols - 8);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = load_group<kT>(x + min(row0 + k, a.rows - 1) * a.ld + col);
+    for (int k = 0; k < 8; ++k) v[k] = load_group<kT>(x + min(row0 + k, a.rows - 1) * a.ld + cl);
+    if (cl != col) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = Group<kT>{};
+    }
   } else {
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] = load_group_edge<kT>(x + min(row0 + k, a.rows - 1) * a.ld, col, a.cols);
