@@ -358,7 +358,8 @@ Tensor gated(const GatedP& w, const Tensor& x, const OptT& add_, int64_t fn, int
     same(x, *add_, what);
     need(add_->scalar_type() == x.scalar_type(), what, "the addend has x's type");
     lead.back() = 2 * w->N;
-    add = add_->expand(lead);  // recorded: the gradient of what is broadcast is summed
+    // expand is recorded: the gradient of what is broadcast is summed
+    add = add_->sizes() == at::IntArrayRef(lead) ? *add_ : add_->expand(lead);
   }
   lead.pop_back();
   if (!records(x) && !(add && records(*add))) return std::get<0>(gated_forward(*w, x, add, fn, fmt, false));

@@ -1,8 +1,8 @@
 // The products of mx4_gemm.hip for at most 16 rows (single tokens, a few conversations): the quantization of x, the
 // product and the gate in one launch.
 //
-// What bounds it: the weight's bytes, read once (17/32 a code), and, for one token, the latency of one launch and of two
-// dependent loads.  A workgroup takes 16 weight rows (gate and up: 16 of each); its waves split K and add their sums
+// What bounds it: the weight's bytes, read once (17/32 a code), and a launch's latency: 1 x 2048 x 6144 in E4M3 takes 4.3 us
+// replayed from a graph, where 1 x 1024 x 1024 takes 2.6 and the weight's bytes at the rate of a large copy 1.3.  A workgroup takes 16 weight rows (gate and up: 16 of each); its waves split K and add their sums
 // through LDS.  One v_mfma_scale_f32_16x16x128 takes a 1 KB weight block as it lies in memory, 16 bytes a lane, with the
 // tokens as the other operand's rows; rows past M repeat the last one.  Its operand of x needs no exchange in E2M1 (lane l
 // holds a whole 32-block of token l % 16) and two lane swaps in E4M3 (each block lies in two lanes), so every wave
@@ -17,8 +17,6 @@
 using namespace mx4;
 
 namespace {
-
-constexpr int kU = 4;  // K tiles in flight in a wave
 
 struct FewArgs {
   const void* x;
@@ -35,9 +33,9 @@ struct FewArgs {
 };
 
 // 16 values of columns k.. of a row, zeros past K
-template <int kT>
+template <int kT, bool kFull>
 __device__ __forceinline__ void load16p(const typename Elem<kT>::T* row, int k, int K, bool vec, Group<kT>* w) {
-  if (vec && k + 16 <= K) {
+  if (kFull || (vec && k + 16 <= K)) {
     w[0] = load_group<kT>(row + k);
     w[1] = load_group<kT>(row + k + 8);
   } else {
@@ -125,46 +123,69 @@ __device__ __forceinline__ void finish(const FewArgs& a, int64_t blk, int lane, 
   store_run<kT, 4>(reinterpret_cast<T*>(a.c) + m * a.ldc, c, a.N, a.vec_c, v);
 }
 
-template <int kT, int kFmt, bool kGated, int kWaves>
+// How a wave comes by the 32 values a lane of a K tile: kEdge element by element where rows are not aligned to 16 bytes or end
+// inside a tile; kDirect from memory; kStaged through LDS, from where a lane's 64 bytes cost no more than their banks (from
+// memory they lie in other lines than its neighbours', 64 lines an instruction).
+enum Source { kEdge, kDirect, kStaged };
+
+template <int kT, int kFmt, bool kGated, int kWaves, int kSrc>
 __global__ __launch_bounds__(64 * kWaves) void few_kernel(const FewArgs a) {
   typedef typename Elem<kT>::T T;
   constexpr int kB = kGated ? 2 : 1;
   __shared__ __attribute__((aligned(16))) f32x4 part[kWaves][kB][64];
+  __shared__ __attribute__((aligned(16))) uint8_t stage[kSrc == kStaged ? kWaves * 4096 : 16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r16 = lane & 15, g = lane >> 4;
   const Rows<kGated> rows(a.b, a.sb, blockIdx.x, a.kt, r16, g);
-  const int per = (a.kt + kWaves - 1) / kWaves, t0 = wave * per, t1 = min(a.kt, t0 + per);
-  const T* xrow = reinterpret_cast<const T*>(a.x) + (int64_t)min(r16, a.M - 1) * a.ld_x;
+  const T* x = reinterpret_cast<const T*>(a.x);
+  const T* xrow = x + (int64_t)min(r16, a.M - 1) * a.ld_x;
   const int k0 = kFmt == MXFP4_E4M3 ? 16 * g : 32 * g, k1 = kFmt == MXFP4_E4M3 ? 64 + 16 * g : 32 * g + 16;
+  // kStaged: 16 rows of 256 bytes; DMA j brings rows 4 j .. 4 j + 3 (lane l row 4 j + l / 16, the 16-byte chunk at place l % 16),
+  // chunk c of row r at place c ^ r, so that 16 rows' reads of one chunk meet every bank.  Rows past M repeat the last one.
+  uint8_t* const mine = stage + (kSrc == kStaged ? wave * 4096 : 0);
+  const T* src[4];
+  if constexpr (kSrc == kStaged) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int r = 4 * j + g;
+      src[j] = x + (int64_t)min(r, a.M - 1) * a.ld_x + ((r16 ^ r) * 8);
+    }
+  }
   v4f acc[kB];
 #pragma unroll
   for (int i = 0; i < kB; ++i) acc[i] = v4f{0.f, 0.f, 0.f, 0.f};
-  for (int t = t0; t < t1; t += kU) {
-    uint4 wv[kU][kB];
-    uint32_t ws[kU][kB];
-    Group<kT> xv[kU][4];
+  for (int t = wave; t < a.kt; t += kWaves) {  // wave w takes K tiles w, w + kWaves, ..
+    uint4 w[kB];
+    uint32_t ws[kB], xs;
+    Group<kT> v[4];
+    if constexpr (kSrc == kStaged) {
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {  // tiles past the wave's range re-read its last one and are not used
-      const int64_t tu = min(t + u, t1 - 1);
+      for (int j = 0; j < 4; ++j)
+        dma16(src[j] + t * 128, lds_addr(mine) + j * 1024);
+    }
 #pragma unroll
-      for (int i = 0; i < kB; ++i) {
-        wv[u][i] = *reinterpret_cast<const uint4*>(rows.w[i] + tu * 1024);
-        ws[u][i] = rows.s[i][tu * 512];
+    for (int i = 0; i < kB; ++i) {
+      w[i] = *reinterpret_cast<const uint4*>(rows.w[i] + (int64_t)t * 1024);
+      ws[i] = rows.s[i][(int64_t)t * 512];
+    }
+    if constexpr (kSrc == kStaged) {
+      wait_vmcnt<0>();  // this wave's own rows
+      asm volatile("" ::: "memory");
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = ((i < 2 ? k0 : k1) >> 3) + (i & 1);
+        v[i].w = *reinterpret_cast<const uint4*>(mine + r16 * 256 + ((c ^ r16) << 4));
       }
+    } else {
+      load16p<kT, kSrc == kDirect>(xrow, t * 128 + k0, a.K, a.vec_x, v);
+      load16p<kT, kSrc == kDirect>(xrow, t * 128 + k1, a.K, a.vec_x, v + 2);
     }
+    const v8i xo = operand<kT, kFmt>(v, g, xs);
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const int tu = min(t + u, t1 - 1);
-      load16p<kT>(xrow, tu * 128 + k0, a.K, a.vec_x, xv[u]);
-      load16p<kT>(xrow, tu * 128 + k1, a.K, a.vec_x, xv[u] + 2);
-    }
-#pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      if (t + u >= t1) break;
-      uint32_t xs;
-      const v8i xo = operand<kT, kFmt>(xv[u], g, xs);
-#pragma unroll
-      for (int i = 0; i < kB; ++i) acc[i] = mma<kFmt>(operand4(wv[u][i]), ws[u][i], xo, xs, acc[i]);
+    for (int i = 0; i < kB; ++i) acc[i] = mma<kFmt>(operand4(w[i]), ws[i], xo, xs, acc[i]);
+    if constexpr (kSrc == kStaged) {
+      __builtin_amdgcn_s_waitcnt(0xc07f);  // its reads, before the next tile's rows come
+      asm volatile("" ::: "memory");
     }
   }
 #pragma unroll
@@ -257,8 +278,15 @@ __global__ __launch_bounds__(512) void thin_kernel(const FewArgs a) {
 
 template <int kT, int kFmt, bool kGated>
 void launch(const FewArgs& a, unsigned blocks, hipStream_t st) {
-  if (a.kt >= 16) few_kernel<kT, kFmt, kGated, 8><<<blocks, 512, 0, st>>>(a);
-  else few_kernel<kT, kFmt, kGated, 4><<<blocks, 256, 0, st>>>(a);
+  // us, 8 / 16 waves: one row E4M3, (N, K) = (2048, 6144) 5.9 / 5.3, (4096, 12288) 10.9 / 9.1, (6144, 2048) 4.3 / 4.3, gated
+  // 4.9 / 5.8.  Direct / staged: 16 rows E2M1, (2048, 6144) 8.6 / 5.3, (6144, 2048) 6.3 / 4.3; 8 rows 6.8 / 5.6 and 5.2 / 5.0; 3
+  // rows 5.4 / 6.2 and 4.2 / 4.9.
+  const bool full = a.vec_x && a.K % 128 == 0, many = a.kt >= 32;
+  if (!full) few_kernel<kT, kFmt, kGated, 8, kEdge><<<blocks, 512, 0, st>>>(a);
+  else if (a.M >= 8 && many) few_kernel<kT, kFmt, kGated, 16, kStaged><<<blocks, 1024, 0, st>>>(a);
+  else if (a.M >= 8) few_kernel<kT, kFmt, kGated, 8, kStaged><<<blocks, 512, 0, st>>>(a);
+  else if (many) few_kernel<kT, kFmt, kGated, 16, kDirect><<<blocks, 1024, 0, st>>>(a);
+  else few_kernel<kT, kFmt, kGated, 8, kDirect><<<blocks, 512, 0, st>>>(a);
 }
 
 template <bool kGated>
