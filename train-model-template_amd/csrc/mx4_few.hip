@@ -205,7 +205,7 @@ __global__ __launch_bounds__(64 * kWaves) void few_kernel(const FewArgs a) {
 // kTB blocks of 16 rows of a quantized operand (a.x its codes, a.sx its scales)
 template <int kT, int kFmt, bool kGated, int kTB>
 __global__ __launch_bounds__(512) void thin_kernel(const FewArgs a) {
-  constexpr int kB = kGated ? 2 : 1, kWaves = 8, kU = 2, kA = kFmt == MXFP4_E4M3 ? 2 : 1;
+  constexpr int kB = kGated ? 2 : 1, kWaves = 8, kA = kFmt == MXFP4_E4M3 ? 2 : 1;
   __shared__ __attribute__((aligned(16))) f32x4 part[kWaves][kB][kTB][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r16 = lane & 15, g = lane >> 4;
@@ -225,39 +225,31 @@ __global__ __launch_bounds__(512) void thin_kernel(const FewArgs a) {
 #pragma unroll
     for (int b = 0; b < kTB; ++b) acc[i][b] = v4f{0.f, 0.f, 0.f, 0.f};
   const int per = (a.kt + kWaves - 1) / kWaves, t0 = wave * per, t1 = min(a.kt, t0 + per);
-  for (int t = t0; t < t1; t += kU) {
-    uint4 wv[kU][kB], xv[kU][kTB][kA];
-    uint32_t ws[kU][kB], xs[kU][kTB];
+  for (int t = t0; t < t1; ++t) {
+    uint4 w[kB], x[kTB][kA];
+    uint32_t ws[kB], xs[kTB];
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const int64_t tu = min(t + u, t1 - 1);
-#pragma unroll
-      for (int i = 0; i < kB; ++i) {
-        wv[u][i] = *reinterpret_cast<const uint4*>(rows.w[i] + tu * 1024);
-        ws[u][i] = rows.s[i][tu * 512];
-      }
-#pragma unroll
-      for (int b = 0; b < kTB; ++b) {
-#pragma unroll
-        for (int h = 0; h < kA; ++h) xv[u][b][h] = *reinterpret_cast<const uint4*>(xp[b] + (tu * kA + h) * 1024);
-        xs[u][b] = xsp[b][tu * 512];
-      }
+    for (int i = 0; i < kB; ++i) {
+      w[i] = *reinterpret_cast<const uint4*>(rows.w[i] + (int64_t)t * 1024);
+      ws[i] = rows.s[i][(int64_t)t * 512];
     }
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      if (t + u >= t1) break;
+    for (int b = 0; b < kTB; ++b) {
 #pragma unroll
-      for (int b = 0; b < kTB; ++b) {
-        v8i x = operand4(xv[u][b][0]);
-        if constexpr (kA == 2) {
-          x[4] = (int)xv[u][b][1].x;
-          x[5] = (int)xv[u][b][1].y;
-          x[6] = (int)xv[u][b][1].z;
-          x[7] = (int)xv[u][b][1].w;
-        }
+      for (int h = 0; h < kA; ++h) x[b][h] = *reinterpret_cast<const uint4*>(xp[b] + ((int64_t)t * kA + h) * 1024);
+      xs[b] = xsp[b][(int64_t)t * 512];
+    }
 #pragma unroll
-        for (int i = 0; i < kB; ++i) acc[i][b] = mma<kFmt>(operand4(wv[u][i]), ws[u][i], x, xs[u][b], acc[i][b]);
+    for (int b = 0; b < kTB; ++b) {
+      v8i xo = operand4(x[b][0]);
+      if constexpr (kA == 2) {
+        xo[4] = (int)x[b][1].x;
+        xo[5] = (int)x[b][1].y;
+        xo[6] = (int)x[b][1].z;
+        xo[7] = (int)x[b][1].w;
       }
+#pragma unroll
+      for (int i = 0; i < kB; ++i) acc[i][b] = mma<kFmt>(operand4(w[i]), ws[i], xo, xs[b], acc[i][b]);
     }
   }
 #pragma unroll

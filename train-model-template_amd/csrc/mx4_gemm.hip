@@ -395,7 +395,7 @@ void gemm_kernel(const GemmArgs g) {
 // products: 256 x 256 tiles with one took 87 us (E2M1, 10752 x 6144 x 2048) and 148 (10752 x 2048 x 12288) where these take 78
 // and 128.  In Tall the E4M3 stages are 64 codes wide, the E2M1 ones 128 (half the barriers).
 template <int kAF>
-using Tall = std::conditional_t<kAF == MXFP4_E4M3, Shape<kAF, 2, 4, 2, 2, 1, 4>, Shape<kAF, 2, 4, 4, 1, 2, 3>>;
+using Tall = Shape<kAF, 2, 4, 4, 1, kAF == MXFP4_E4M3 ? 1 : 2, 3>;  // 256 x 128, 65 or 76 KB
 template <int kAF>
 using Mid = Shape<kAF, 2, 2, 2, 2, 2, kAF == MXFP4_E4M3 ? 3 : 4>;  // 128 x 128, 75 or 68 KB
 template <int kAF>
