@@ -283,15 +283,15 @@ void distill_kernel(const Args a) {
       }
     }
     if constexpr (kStream) {
-    int v = tid + kHold * kThreads;
-    for (; v + 3 * kThreads < pv; v += 4 * kThreads) {
-      uint4 x[4];
+      int v = tid + kHold * kThreads;
+      for (; v + 3 * kThreads < pv; v += 4 * kThreads) {
+        uint4 x[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) x[u] = load(v + u * kThreads);
+        for (int u = 0; u < 4; ++u) x[u] = load(v + u * kThreads);
 #pragma unroll
-      for (int u = 0; u < 4; ++u) vector(v + u * kThreads, x[u]);
-    }
-    for (; v < pv; v += kThreads) vector(v, load(v));
+        for (int u = 0; u < 4; ++u) vector(v + u * kThreads, x[u]);
+      }
+      for (; v < pv; v += kThreads) vector(v, load(v));
     }
   } else {
     for (int i = tid; i < a.parts; i += kThreads) {
@@ -331,34 +331,34 @@ void distill_kernel(const Args a) {
     if (!vec) {  // the gradient lies otherwise in its 16 bytes than the logits (so it is not in place)
       for (int64_t j = c0 + tid; j < c1; j += kThreads) g[j] = Elem<kT>::put(value(Elem<kT>::get(z[j])));
     } else {
-    if (first && tid < head) g[tid] = Elem<kT>::put(value(Elem<kT>::get(z[tid])));
-    if (last && tail0 + tid < a.V) g[tail0 + tid] = Elem<kT>::put(value(Elem<kT>::get(z[tail0 + tid])));
-    char* const gp = reinterpret_cast<char*>(g + head + v0 * n);
-    auto out = [&](int v, uint4 raw) {
-      float x[n];
-      unpack_vec<kT>(raw, x);
+      if (first && tid < head) g[tid] = Elem<kT>::put(value(Elem<kT>::get(z[tid])));
+      if (last && tail0 + tid < a.V) g[tail0 + tid] = Elem<kT>::put(value(Elem<kT>::get(z[tail0 + tid])));
+      char* const gp = reinterpret_cast<char*>(g + head + v0 * n);
+      auto out = [&](int v, uint4 raw) {
+        float x[n];
+        unpack_vec<kT>(raw, x);
 #pragma unroll
-      for (int i = 0; i < n; ++i) x[i] = value(x[i]);
-      store_codes<true>(reinterpret_cast<uint8_t*>(gp + (uint32_t)v * 16u), pack_vec<kT>(x));
-    };
-    if constexpr (kHold > 0) {
+        for (int i = 0; i < n; ++i) x[i] = value(x[i]);
+        store_codes<true>(reinterpret_cast<uint8_t*>(gp + (uint32_t)v * 16u), pack_vec<kT>(x));
+      };
+      if constexpr (kHold > 0) {
 #pragma unroll
-      for (int u = 0; u < kHold; ++u) {
-        if (tid + u * kThreads < pv) out(tid + u * kThreads, held[u]);
-        __builtin_amdgcn_sched_barrier(0);
+        for (int u = 0; u < kHold; ++u) {
+          if (tid + u * kThreads < pv) out(tid + u * kThreads, held[u]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
-    }
-    if constexpr (kStream) {
-    int v = tid + kHold * kThreads;
-    for (; v + 3 * kThreads < pv; v += 4 * kThreads) {
-      uint4 x[4];
+      if constexpr (kStream) {
+        int v = tid + kHold * kThreads;
+        for (; v + 3 * kThreads < pv; v += 4 * kThreads) {
+          uint4 x[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) x[u] = load(v + u * kThreads);
+          for (int u = 0; u < 4; ++u) x[u] = load(v + u * kThreads);
 #pragma unroll
-      for (int u = 0; u < 4; ++u) out(v + u * kThreads, x[u]);
-    }
-    for (; v < pv; v += kThreads) out(v, load(v));
-    }
+          for (int u = 0; u < 4; ++u) out(v + u * kThreads, x[u]);
+        }
+        for (; v < pv; v += kThreads) out(v, load(v));
+      }
     }
     if (zero) return;
     __syncthreads();  // this workgroup's stores have completed: S goes over them
@@ -431,7 +431,8 @@ extern "C" int distill_topk_kl(const void* logits, int64_t type, int64_t ld, int
   MX_CHECK_ARG(tau > 0.f && tau < __builtin_inff(), "distill_topk_kl: the temperature has to be positive");
   MX_CHECK_ARG(parts >= 1 && parts <= DISTILL_MAX_PARTS && stages >= 1 && stages <= 3, "distill_topk_kl: bad plan");
   if (T == 0) return MXFP8_OK;
-  MX_CHECK_ARG(T * parts < (1LL << 31), "distill_topk_kl: too many rows");
+  MX_CHECK_ARG(T < (1LL << 31) && T * parts * 1024 < (1LL << 32) * (V <= 4096 && parts == 1 ? 4 : 1),
+               "distill_topk_kl: more rows than one launch has threads for (T=%lld)", (long long)T);
   const bool whole = stages == 3 && parts == 1;
   MX_CHECK_ARG(logits && idx && t && (whole || ws) && (loss || grad || stages == DISTILL_STATS),
                "distill_topk_kl: null pointer");

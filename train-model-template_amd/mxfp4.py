@@ -9,14 +9,20 @@ that).  Everything runs in the hand-written kernels of libmxfp8_mlp.so; a CPU te
     y = mxfp4.mx4_linear(x, W)                 # [.., N]; autograd gives dx, the weight is frozen
     G = mxfp4.GatedWeight(gate.weight, up.weight)
     h = mxfp4.mx4_gated(x, G)                  # silu(x Wgᵀ) * (x Wuᵀ)
+    mxfp4.enable_mxfp4(model)                  # or a whole model's frozen linears and gated MLPs, adapters kept
 
 Block scale: with amax the largest magnitude of the block and max = 6 (E2M1) or 448 (E4M3), the least power of two e with
 amax <= max e (so nothing is clipped), 2^-127 at the least; codes round to nearest, ties to even.  A NaN makes its block
 NaN; an infinity takes the format's largest value times 2^127.  Sums are fp32, with one rounding to the output's type.
 """
+import types
+
 import torch
+from torch import nn
 
 import _native
+import mxfp8
+from fused_linear import _part
 
 E2M1, E4M3 = 4, 8
 _FMT = {"e2m1": E2M1, "e4m3": E4M3}
@@ -120,3 +126,98 @@ def mx4_gated(x, w, add=None, fn="silu", act="e4m3"):
     if fn not in _FN:
         raise ValueError(f"unknown gate function {fn!r}: one of {sorted(_FN)}")
     return _native.host4().gated(w.handle, x, add, _FN[fn], _FMT.get(act) or _fmt(act))
+
+
+# ---------------------------------------------------------------- a model's frozen linears
+_SILU, _GELU = ("SiLU", "SiLUActivation"), ("GELUTanh", "PytorchGELUTanh")
+
+
+def _gate_name(mlp):
+    """The gate function of a gated MLP module, or None for one that mx4_gated does not have."""
+    f = getattr(mlp, "act_fn", None)
+    name = type(f).__name__
+    if name in _SILU:
+        return "silu"
+    return "gelu" if name in _GELU or (isinstance(f, nn.GELU) and f.approximate == "tanh") else None
+
+
+def _lora(proj):
+    """_part, and the base layer alone where the adapters are switched off for a while."""
+    part = _part(proj)
+    off = part is None and getattr(proj, "disable_adapters", False) and not proj.merged
+    return (proj.base_layer, None, None, 1.0) if off else part
+
+
+def _adapter(x, part):
+    """An adapter's output s (x Aᵀ) Bᵀ in x's type, or None."""
+    _, A, B, s = part
+    return None if A is None else ((x @ A.to(x.dtype).t()) @ B.to(x.dtype).t()) * s
+
+
+def mlp(mod, x):
+    """down(fn(gate(x)) * up(x)) of a gated MLP that enable_mxfp4 took: one gated block over the gate and up weights with
+    their adapters' outputs added before the gate, and one linear."""
+    G, D, fn, act = mod._mx4_gated
+    parts = [_lora(getattr(mod, n)) for n in ("gate_proj", "up_proj", "down_proj")]
+    if None in parts:
+        raise ValueError("mxfp4.mlp: gate, up and down take plain frozen linears or one LoRA adapter without dropout, unmerged")
+    g, u = _adapter(x, parts[0]), _adapter(x, parts[1])
+    add = None
+    if g is not None or u is not None:
+        zero = x.new_zeros(())
+        wide = (*x.shape[:-1], G.shape[0])
+        add = torch.cat([zero.expand(wide) if t is None else t for t in (g, u)], -1)
+    h = mx4_gated(x, G, add=add, fn=fn, act=act)
+    y = mx4_linear(h, D, act=act)
+    d = _adapter(h, parts[2])
+    return y if d is None else y + d
+
+
+def _linear_forward(self, x):
+    W, act = self._mx4
+    if W is None:
+        raise RuntimeError("this projection is held by its MLP's gated block (mxfp4.enable_mxfp4) and has no call of its own")
+    return mx4_linear(x, W, act=act)
+
+
+def enable_mxfp4(model, act="e4m3"):
+    """Quantize every frozen base linear of the decoder layers (those of mxfp8.enable_mxfp8: any shape here, no bias) to
+    MXFP4 along both axes, move the weights to host memory and route the layers' forward through mx4_linear.  An MLP with
+    gate_proj, up_proj, down_proj and a SiLU or tanh-GELU act_fn runs as `mlp` instead, if its adapters let it.  LoRA wrappers
+    keep working: their base layer is what changes.  Returns the number of linears."""
+    _fmt(act)  # refuses an unknown name before anything is touched
+    found = {id(lin): lin for _, lin in mxfp8._base_linears(model)}
+    for lin in found.values():
+        if lin.bias is not None or mxfp8.is_mx(lin) or "_mx4" in lin.__dict__:
+            raise ValueError("enable_mxfp4: linears without bias that are not quantized yet")
+    held = {}
+    for mod in model.modules():
+        projs = [getattr(mod, n, None) for n in ("gate_proj", "up_proj", "down_proj")]
+        if None in projs or _gate_name(mod) is None or None in [_lora(p) for p in projs]:
+            continue
+        base = [getattr(p, "base_layer", p) for p in projs]
+        if all(id(b) in found for b in base) and base[0].weight.shape == base[1].weight.shape \
+                and base[0].weight.dtype == base[1].weight.dtype:
+            G, D = GatedWeight(base[0].weight, base[1].weight), Weight(base[2].weight)
+            mod._mx4_gated = (G, D, _gate_name(mod), act)
+            mod.forward = types.MethodType(mlp, mod)
+            held.update({id(base[0]): None, id(base[1]): None, id(base[2]): D})
+    for lin in found.values():
+        w = lin.weight.data
+        lin._mx4 = (held[id(lin)] if id(lin) in held else Weight(w), act)
+        lin._bf16_cpu = w.to("cpu", copy=True)
+        lin.weight.data = torch.empty((0,), dtype=w.dtype, device=w.device)
+        lin.forward = types.MethodType(_linear_forward, lin)
+    torch.cuda.empty_cache()
+    return len(found)
+
+
+def disable_mxfp4(model):
+    """Put the weights back on their device and take the 4-bit copies and the patched forwards away."""
+    for mod in model.modules():
+        if "_mx4_gated" in mod.__dict__:
+            del mod._mx4_gated, mod.forward
+        if "_mx4" in mod.__dict__:
+            mod.weight.data = mod._bf16_cpu.to(mod.weight.device)
+            del mod._mx4, mod._bf16_cpu, mod.forward
+    torch.cuda.empty_cache()
