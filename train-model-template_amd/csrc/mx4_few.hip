@@ -298,8 +298,8 @@ int run(FewArgs& a, int64_t fmt, int64_t type, const char* what, hipStream_t st)
 
 template <int kT, int kFmt, bool kGated>
 void launch_thin(const FewArgs& a, unsigned blocks, hipStream_t st) {
-  if (a.M <= 32) thin_kernel<kT, kFmt, kGated, 2><<<blocks, 512, 0, st>>>(a);
-  else thin_kernel<kT, kFmt, kGated, 4><<<blocks, 512, 0, st>>>(a);
+  if (kFmt == MXFP4_E4M3 || a.M <= 32) thin_kernel<kT, kFmt, kGated, 2><<<blocks, 512, 0, st>>>(a);  // 32 rows at most in E4M3
+  else thin_kernel<kT, kFmt, kGated, kFmt == MXFP4_E4M3 ? 2 : 4><<<blocks, 512, 0, st>>>(a);
 }
 template <bool kGated>
 void run_thin(const FewArgs& a, int64_t fmt, int64_t type, hipStream_t st) {

@@ -26,6 +26,7 @@ namespace {
 template <int kAF_, int kMB_, int kNB_, int kWM_, int kWN_, int kKS_, int kStages_>
 struct Shape {
   static constexpr int kAF = kAF_, kMB = kMB_, kNB = kNB_, kWM = kWM_, kWN = kWN_, kKS = kKS_, kStages = kStages_;
+  static constexpr bool kDeep = kMB * kNB <= 4;  // registers for a whole K tile's fragments ahead
   static constexpr int kWaves = kWM * kWN, kThreads = 64 * kWaves;
   static constexpr int kBM = 32 * kMB * kWM, kBN = 32 * kNB * kWN;
   static constexpr int kGroupM = 1024 / kBM;                                      // M-tiles of a tile group
@@ -320,9 +321,62 @@ void gemm_kernel(const GemmArgs g) {
   using H0 = std::integral_constant<int, 0>;
   using H1 = std::integral_constant<int, 1>;
 
-  Frags f0, f1;
   int slot = 0;  // ring slot of the stage at hand
-  if constexpr (S::kKS == 2) {
+  if constexpr (S::kDeep) {
+    // The fragments of a whole K tile are read while the products of the one before run, so the LDS's latency is paid beside
+    // them.  At the barrier of tile s every wave has read tile s, whose slot takes tile s + kStages.
+    struct Tile {
+      Frags f[2];
+      uint32_t sa[kMB], sb[kNB];
+    };
+    Tile t0, t1;
+    auto read_tile = [&](int sl, Tile& t, int r) {
+      if (r == 0) {
+        read_words<kMB>(lds + sl * S::kStageBytes + sao, t.sa);
+        read_words<kNB>(lds + sl * S::kStageBytes + sbo, t.sb);
+      }
+      read_frag(sl, r / kReads, t.f[r / kReads], r % kReads);
+    };
+#pragma unroll
+    for (int q = 0; q < S::kStages; ++q)
+#pragma unroll
+      for (int d = 0; d < S::kDma; ++d) dma(min(q, last), q, d);
+    wait_vmcnt<(S::kStages - 1) * S::kDma>();
+    stage_barrier();
+#pragma unroll
+    for (int r = 0; r < 2 * kReads; ++r) read_tile(0, t0, r);
+    auto one = [&](int s, Tile& cur, Tile& nxt) {
+      wait_vmcnt<(S::kStages - 2) * S::kDma>();
+      __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): this wave's reads of tile s are in registers
+      stage_barrier();
+      const int old = slot;
+      slot = slot + 1 == S::kStages ? 0 : slot + 1;
+#pragma unroll
+      for (int i = 0; i < kMB; ++i) sca[i] = cur.sa[i] >> sshift;
+#pragma unroll
+      for (int i = 0; i < kNB; ++i) scb[i] = cur.sb[i] >> sshift;
+      constexpr int kAll = 2 * kMfma, kOver = kAll - 1;
+#pragma unroll
+      for (int x = 0; x < kAll; ++x) {
+        if (x < kMfma) mma(cur.f[0], x, H0{});
+        else mma(cur.f[1], x - kMfma, H1{});
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int r = 0; r < 2 * kReads; ++r)
+          if (r * kOver / (2 * kReads) == x) read_tile(slot, nxt, r);
+#pragma unroll
+        for (int d = 0; d < S::kDma; ++d)
+          if (d * kOver / S::kDma == x) dma(min(s + S::kStages, last), old, d);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    int s = 0;
+    for (; s < last; s += 2) {
+      one(s, t0, t1);
+      one(s + 1, t1, t0);
+    }
+    if (s == last) one(s, t0, t1);
+  } else if constexpr (S::kKS == 2) {
     // K tile s frees its ring slot at the barrier in its second half; that half and the first half of tile s + 1 refill it
     // with tile s + kStages.  So the ring starts with the second part of its last stage still to come.  Tiles past the end
     // re-load the last one into slots that nothing reads any more: the number in flight is the same at every wait.
@@ -333,6 +387,7 @@ void gemm_kernel(const GemmArgs g) {
     wait_vmcnt<(S::kStages - 2) * S::kDma + kD0>();
     stage_barrier();
     read_scales(0);
+    Frags f0, f1;
 #pragma unroll
     for (int r = 0; r < kReads; ++r) read_frag(0, 0, f0, r);
     int pslot = S::kStages - 1;  // of the tile before
@@ -356,6 +411,7 @@ void gemm_kernel(const GemmArgs g) {
     wait_vmcnt<(S::kStages - 1) * S::kDma>();
     stage_barrier();
     read_scales(0);
+    Frags f0, f1;
 #pragma unroll
     for (int r = 0; r < kReads; ++r) read_frag(0, 0, f0, r);
     auto one = [&](int s, Frags& cur, Frags& nxt, auto half) {
@@ -393,13 +449,17 @@ void gemm_kernel(const GemmArgs g) {
 
 // Every ring leaves room for two workgroups a CU, so that one's pipeline fill, barriers and epilogue overlap the other's
 // products: 256 x 256 tiles with one took 87 us (E2M1, 10752 x 6144 x 2048) and 148 (10752 x 2048 x 12288) where these take 78
-// and 128.  In Tall the E4M3 stages are 64 codes wide, the E2M1 ones 128 (half the barriers).
+// and 128.  In Tall the E4M3 stages are 64 codes wide, the E2M1 ones 128 (half the barriers).  The others hold a whole K
+// tile's fragments ahead, for which Tall has no registers left: at 1000 x 1024 x 7168 in E4M3 that took Low from 16.3 to 14.2
+// us, Mid from 22.0 to 20.4, and Mini (twice Low's workgroups where those leave CUs idle) from 14.6 to 13.6.
 template <int kAF>
 using Tall = Shape<kAF, 2, 4, 4, 1, kAF == MXFP4_E4M3 ? 1 : 2, 3>;  // 256 x 128, 65 or 76 KB
 template <int kAF>
 using Mid = Shape<kAF, 2, 2, 2, 2, 2, kAF == MXFP4_E4M3 ? 3 : 4>;  // 128 x 128, 75 or 68 KB
 template <int kAF>
 using Low = Shape<kAF, 1, 2, 2, 2, 2, 4>;  // 64 x 128, 68 or 52 KB
+template <int kAF>
+using Mini = Shape<kAF, 1, 1, 2, 2, 2, 4>;  // 64 x 64, 52 or 36 KB
 
 template <class S, int kEpi>
 int launch(GemmArgs& g, const char* what, hipStream_t st) {
@@ -416,13 +476,15 @@ int launch(GemmArgs& g, const char* what, hipStream_t st) {
 
 template <int kEpi, int kAF>
 int dispatch(GemmArgs& g, const char* what, hipStream_t st) {
-  switch (mx4_shape(g.M, g.rows_b, g.kt, kAF == MXFP4_E4M3, g.b_pi && g.type != MXFP4_F32 && !g.gu, 256)) {
+  switch (mx4_shape(g.M, g.rows_b, g.kt, kAF == MXFP4_E4M3, kEpi == kGated, g.b_pi && g.type != MXFP4_F32 && !g.gu, 256)) {
     case kMx4Thin:
       mx4_thin(kEpi == kGated, g.a, g.sa, kAF, g.b, g.sb, g.M, g.N, g.kt, g.add, g.ld_add, g.fn, g.c, g.ldc, g.type, st);
       MX_CHECK_LAUNCH(what);
       return MXFP8_OK;
     case kMx4Tall: return launch<Tall<kAF>, kEpi>(g, what, st);
     case kMx4Mid: return launch<Mid<kAF>, kEpi>(g, what, st);
+    case kMx4Mini:
+      if constexpr (kEpi == kPlain) return launch<Mini<kAF>, kEpi>(g, what, st);
     default: return launch<Low<kAF>, kEpi>(g, what, st);
   }
 }
