@@ -2,9 +2,12 @@
 // from fp32 into the operand of the product with [W_gate; W_up] (and, where an addend wants its gradient, rounded to the
 // activations' type).
 //
-// What bounds it: memory, 6 bytes read and 2 (E4M3) or 1 (E2M1) written for each column of a row.  The saved values lie in
-// the order of the forward epilogue's lanes, which is this kernel's order too: lane l of a wave holds row l % 32 and 16
-// columns of a 32 x 32 block, a 32-column scale block is two lanes, and every load of the saved values is 1 KB in a row.
+// What bounds it: memory, 6 bytes read and 2 (E4M3) or 1 (E2M1) written for each column of a row, and 4 more for the addend's
+// gradient: 10752 x 6144 bf16 in E4M3 takes 90 us, 188 with the addend's gradient (5.9 and 4.2 TB/s; part of it comes from the
+// last-level cache).  The saved values lie in the order of the forward epilogue's lanes, which is this kernel's order too:
+// lane l of a wave holds row l % 32 and 16 columns of a 32 x 32 block, a 32-column scale block is two lanes, and every load of
+// the saved values is 1 KB in a row.  One block a wave: four in a row, each asked for while the one before was computed, took
+// 98 and 206 us, and 15.2 where this takes 12.5 at 1000 x 3584, whose waves then waited four times for memory.
 #include "abi_common.h"
 #include "mx4_device.h"
 
@@ -48,51 +51,39 @@ __device__ __forceinline__ uint32_t quant_store(const float* v, int64_t m, int64
   return live ? e : 0u;
 }
 
+// A workgroup takes 32 rows and 128 columns, a wave a 32 x 32 block of them.  Rows up to the scale tiles' 128 take part, so that
+// all scale bytes are written.
 template <int kT, int kFn, int kFmt>
 __global__ __launch_bounds__(kThreads) void gate_bwd_kernel(const BwdArgs a) {
   typedef typename Elem<kT>::T T;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, hi = lane >> 5;
-  const int64_t nblk = (a.N + 31) / 32, tiles = (a.N + 127) / 128;
-  const int64_t m = (int64_t)blockIdx.y * 128 + w * 32 + (lane & 31);  // scale bytes of a tile's 128 rows are all written
-  const int64_t mc = min(m, (int64_t)a.M - 1);
+  const int64_t nblk = (a.N + 31) / 32;
+  const uint32_t tiles = (uint32_t)(a.N + 127) / 128, rb = blockIdx.x / tiles, tile = blockIdx.x - rb * tiles;
+  const int64_t m = (int64_t)rb * 32 + (lane & 31), mc = min(m, (int64_t)a.M - 1);
   const bool live = m < a.M;
-  uint32_t sg = 0, su = 0;  // the row's four scale bytes of the gate's and the up's tile
-  const T* const sv = reinterpret_cast<const T*>(a.gu);
-  const T* const p = reinterpret_cast<const T*>(a.dh) + mc * a.ld_dh;
-  struct Raw {
-    Group<kT> g[2], u[2], d[2];
-  };
-  // a block's values, asked for while the block before is computed; saved values are read once and pass the caches by
-  auto load = [&](int b) {
-    Raw r;
-    const int64_t cb = min((int64_t)blockIdx.x * 128 + b * 32, (nblk - 1) * 32), c = cb + hi * 16;
-    const T* s = sv + saved_offset(mc, c, nblk);
-    r.g[0].w = load_nt(s);
-    r.g[1].w = load_nt(s + 512);
-    r.u[0].w = load_nt(s + 1024);
-    r.u[1].w = load_nt(s + 1536);
+  const int64_t cb = (int64_t)tile * 128 + w * 32, c = cb + hi * 16;
+  float dg[16], du[16];
+  if (cb < a.N) {
+    Group<kT> gr[2], ur[2], dr[2];
+    const T* s = reinterpret_cast<const T*>(a.gu) + saved_offset(mc, c, nblk);
+    gr[0].w = load_nt(s);  // read once: past the caches
+    gr[1].w = load_nt(s + 512);
+    ur[0].w = load_nt(s + 1024);
+    ur[1].w = load_nt(s + 1536);
+    const T* p = reinterpret_cast<const T*>(a.dh) + mc * a.ld_dh;
     if (a.vec_dh && cb + 32 <= a.N) {
-      r.d[0] = load_group<kT>(p + c);
-      r.d[1] = load_group<kT>(p + c + 8);
+      dr[0] = load_group<kT>(p + c);
+      dr[1] = load_group<kT>(p + c + 8);
     } else {
-      r.d[0] = load_group_edge<kT>(p, c, a.N);
-      r.d[1] = load_group_edge<kT>(p, c + 8, a.N);
+      dr[0] = load_group_edge<kT>(p, c, a.N);
+      dr[1] = load_group_edge<kT>(p, c + 8, a.N);
     }
-    return r;
-  };
-  Raw cur = load(0);
-#pragma unroll
-  for (int b = 0; b < 4; ++b) {
-    const int64_t cb = (int64_t)blockIdx.x * 128 + b * 32, c = cb + hi * 16;
-    const Raw raw = cur;
-    if (b < 3) cur = load(b + 1);
-    float dg[16], du[16];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       float g[8], u[8], d[8];
-      raw.g[h].values(g);
-      raw.u[h].values(u);
-      raw.d[h].values(d);
+      gr[h].values(g);
+      ur[h].values(u);
+      dr[h].values(d);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         float df;
@@ -101,27 +92,27 @@ __global__ __launch_bounds__(kThreads) void gate_bwd_kernel(const BwdArgs a) {
         du[8 * h + i] = d[i] * f;
       }
     }
-    if (cb + 32 > a.N) {  // the saved values past the last column are undefined
+  }
+  if (cb + 32 > a.N) {  // the saved values past the last column are undefined
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        dg[i] = c + i < a.N ? dg[i] : 0.f;
-        du[i] = c + i < a.N ? du[i] : 0.f;
-      }
-    }
-    sg |= quant_store<kFmt>(dg, m, c, 2 * tiles, live, a.q) << (8 * b);
-    su |= quant_store<kFmt>(du, m, tiles * 128 + c, 2 * tiles, live, a.q) << (8 * b);
-    if (a.dgu && live) {
-      T* o = reinterpret_cast<T*>(a.dgu) + m * 2 * a.N;
-      store_run<kT, 16>(o, c, a.N, a.vec_dgu, dg);
-      store_run<kT, 16>(o + a.N, c, a.N, a.vec_dgu, du);
+    for (int i = 0; i < 16; ++i) {
+      dg[i] = c + i < a.N ? dg[i] : 0.f;
+      du[i] = c + i < a.N ? du[i] : 0.f;
     }
   }
-  const int64_t t = (int64_t)blockIdx.y * 2 * tiles + blockIdx.x + (hi ? tiles : 0);
-  *reinterpret_cast<uint32_t*>(a.s + t * 512 + (lane & 31) * 16 + w * 4) = hi ? su : sg;
+  const uint32_t sg = quant_store<kFmt>(dg, m, c, 2 * tiles, live, a.q);
+  const uint32_t su = quant_store<kFmt>(du, m, (int64_t)tiles * 128 + c, 2 * tiles, live, a.q);
+  const int64_t t = (int64_t)(rb >> 2) * 2 * tiles + tile + (hi ? tiles : 0);
+  a.s[t * 512 + (lane & 31) * 16 + (rb & 3) * 4 + w] = (uint8_t)(hi ? su : sg);
+  if (a.dgu && live) {
+    T* o = reinterpret_cast<T*>(a.dgu) + m * 2 * a.N;
+    store_run<kT, 16>(o, c, a.N, a.vec_dgu, dg);
+    store_run<kT, 16>(o + a.N, c, a.N, a.vec_dgu, du);
+  }
 }
 
 template <int kT, int kFn>
-void launch(const BwdArgs& a, int64_t fmt, dim3 grid, hipStream_t st) {
+void launch(const BwdArgs& a, int64_t fmt, unsigned grid, hipStream_t st) {
   if (fmt == MXFP4_E4M3) gate_bwd_kernel<kT, kFn, MXFP4_E4M3><<<grid, kThreads, 0, st>>>(a);
   else gate_bwd_kernel<kT, kFn, MXFP4_E2M1><<<grid, kThreads, 0, st>>>(a);
 }
@@ -139,10 +130,11 @@ extern "C" int mxfp4_gated_bwd(const void* gu, const void* dh, int64_t ld_dh, in
   MX_CHECK_ARG(gu && dh && q && s && ld_dh >= N, "mxfp4_gated_bwd: null pointer or bad stride");
   MX_CHECK_ARG(mx_aligned(gu, 16) && mx_aligned(dh, 2) && mx_aligned(q, 16) && mx_aligned(s, 16) && mx_aligned(dgu, 2),
                "mxfp4_gated_bwd: misaligned buffer");
-  MX_CHECK_ARG((M + 127) / 128 <= 65535, "mxfp4_gated_bwd: too many rows");
+  const int64_t wgs = (N + 127) / 128 * ((M + 127) / 128 * 4);
+  MX_CHECK_ARG(wgs < (1 << 24), "mxfp4_gated_bwd: too large (M=%lld N=%lld)", (long long)M, (long long)N);
   const BwdArgs a{gu, dh, ld_dh, (int)M, (int)N, (uint8_t*)q, (uint8_t*)s, dgu, mx_aligned(dh, 16) && ld_dh % 8 == 0,
                   mx_aligned(dgu, 16) && N % 8 == 0};
-  const dim3 grid((unsigned)((N + 127) / 128), (unsigned)((M + 127) / 128));
+  const unsigned grid = (unsigned)wgs;
   const hipStream_t st = (hipStream_t)stream;
   if (type == MXFP4_BF16)
     fn == MXFP4_SILU ? launch<MXFP4_BF16, MXFP4_SILU>(a, fmt, grid, st) : launch<MXFP4_BF16, MXFP4_GELU>(a, fmt, grid, st);
