@@ -324,6 +324,36 @@ __device__ __forceinline__ void store_run(typename Elem<kT>::T* p, int64_t c, in
     if (c + i < cols) p[c + i] = Elem<kT>::put(v[i]);
 }
 
+// Columns c0 .. c0 + 31 of rows r0 .. r0 + 31 from a wave whose lane l holds, of row l % 32, the 16 columns at (l / 32) 16.  In 16
+// bits the lanes l and l ^ 16 swap halves first, so that an instruction writes 16 rows of 64 bytes and not 32 of 16 in each of
+// two places.  r0, c0 are the same in all lanes, all of which call it.
+template <int kT>
+__device__ __forceinline__ void store_block(typename Elem<kT>::T* p, int64_t ld, int64_t r0, int64_t rows, int64_t c0,
+                                            int64_t cols, bool vec, int lane, const float* v) {
+  if constexpr (kT != MXFP4_F32) {
+    if (vec && c0 + 32 <= cols) {
+      uint32_t w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float a = v[2 * i], b = v[2 * i + 1];
+        w[i] = round2<kT>(a, b);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {  // now w[0..3] row l % 16, w[4..7] row 16 + l % 16, columns 8 (l / 16 % 2) of the 16
+        const auto r = __builtin_amdgcn_permlane16_swap(w[i], w[4 + i], false, false);
+        w[i] = r[0];
+        w[4 + i] = r[1];
+      }
+      const int64_t c = c0 + (lane >> 5) * 16 + ((lane >> 4) & 1) * 8, r = r0 + (lane & 15);
+      if (r < rows) *reinterpret_cast<uint4*>(p + r * ld + c) = make_uint4(w[0], w[1], w[2], w[3]);
+      if (r + 16 < rows) *reinterpret_cast<uint4*>(p + (r + 16) * ld + c) = make_uint4(w[4], w[5], w[6], w[7]);
+      return;
+    }
+  }
+  const int64_t r = r0 + (lane & 31);
+  if (r < rows) store_run<kT, 16>(p + r * ld, c0 + (lane >> 5) * 16, cols, vec, v);
+}
+
 // ---- gate functions: f = fn(g); and its derivative
 // silu(g) = g s, s = 1 / (1 + exp(-g)); silu' = s (1 + g (1 - s)).
 // gelu(g) = g s(2 c (g + a g^3)) with c = sqrt(2 / pi), a = 0.044715 (0.5 (1 + tanh t) = sigmoid(2 t)), so

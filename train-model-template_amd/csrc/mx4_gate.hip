@@ -104,10 +104,10 @@ __global__ __launch_bounds__(kThreads) void gate_bwd_kernel(const BwdArgs a) {
   const uint32_t su = quant_store<kFmt>(du, m, (int64_t)tiles * 128 + c, 2 * tiles, live, a.q);
   const int64_t t = (int64_t)(rb >> 2) * 2 * tiles + tile + (hi ? tiles : 0);
   a.s[t * 512 + (lane & 31) * 16 + (rb & 3) * 4 + w] = (uint8_t)(hi ? su : sg);
-  if (a.dgu && live) {
-    T* o = reinterpret_cast<T*>(a.dgu) + m * 2 * a.N;
-    store_run<kT, 16>(o, c, a.N, a.vec_dgu, dg);
-    store_run<kT, 16>(o + a.N, c, a.N, a.vec_dgu, du);
+  if (a.dgu) {
+    T* o = reinterpret_cast<T*>(a.dgu);
+    store_block<kT>(o, 2 * (int64_t)a.N, rb * 32, a.M, cb, a.N, a.vec_dgu, lane, dg);
+    store_block<kT>(o + a.N, 2 * (int64_t)a.N, rb * 32, a.M, cb, a.N, a.vec_dgu, lane, du);
   }
 }
 

@@ -114,14 +114,14 @@ __device__ __forceinline__ void store_plain(const GemmArgs& g, int m0, int n0, i
 #pragma unroll
     for (int mt = 0; mt < S::kMB; ++mt) {
       const int m = m0 + mt * 32 + (lane & 31), nb = n0 + nt * 32;
-      if (m >= g.M || nb >= g.N) continue;
-      T* row = reinterpret_cast<T*>(g.c) + (int64_t)m * g.ldc;
+      if (nb >= g.N) continue;
       float v[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) v[i] = acc[nt][mt][i];
       if (g.b_pi) {
-        store_run<kT, 16>(row, nb + (lane >> 5) * 16, g.N, g.vec, v);
-      } else {
+        store_block<kT>(reinterpret_cast<T*>(g.c), g.ldc, m0 + mt * 32, g.M, nb, g.N, g.vec, lane, v);
+      } else if (m < g.M) {
+        T* row = reinterpret_cast<T*>(g.c) + (int64_t)m * g.ldc;
 #pragma unroll
         for (int q = 0; q < 4; ++q) store_run<kT, 4>(row, nb + q * 8 + (lane >> 5) * 4, g.N, g.vec, v + 4 * q);
       }
@@ -157,9 +157,10 @@ __device__ __forceinline__ void store_gated(const GemmArgs& g, int m0, int n0, i
   for (int p = 0; p < S::kNB / 2; ++p)
 #pragma unroll
     for (int mt = 0; mt < S::kMB; ++mt) {
-      const int m = m0 + mt * 32 + (lane & 31);
-      const int c = (n0 >> 1) + p * 32 + (lane >> 5) * 16;  // the lane's first gate and up column
-      if (m >= g.M || (n0 >> 1) + p * 32 >= g.N) continue;
+      // rows past the last one compute the last one's and are not stored
+      const int m = min(m0 + mt * 32 + (lane & 31), g.M - 1), c0 = (n0 >> 1) + p * 32;
+      const int c = c0 + (lane >> 5) * 16;  // the lane's first gate and up column
+      if (c0 >= g.N) continue;
       float gv[16], uv[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
@@ -175,7 +176,7 @@ __device__ __forceinline__ void store_gated(const GemmArgs& g, int m0, int n0, i
 #pragma unroll
         for (int i = 0; i < 16; ++i) uv[i] += t[i];
       }
-      if (g.gu) {
+      if (g.gu && m0 + mt * 32 + (lane & 31) < g.M) {
         T* s = reinterpret_cast<T*>(g.gu) + saved_offset(m, c, nblk);
         // read again by the backward pass alone: past the caches, which keep h
         store_nt8<kT>(s, gv);
@@ -185,7 +186,7 @@ __device__ __forceinline__ void store_gated(const GemmArgs& g, int m0, int n0, i
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) gv[i] = gate_fn<kFn>(gv[i]) * uv[i];
-      store_run<kT, 16>(reinterpret_cast<T*>(g.c) + (int64_t)m * g.ldc, c, g.N, g.vec, gv);
+      store_block<kT>(reinterpret_cast<T*>(g.c), g.ldc, m0 + mt * 32, g.M, c0, g.N, g.vec, lane, gv);
     }
 }
 
