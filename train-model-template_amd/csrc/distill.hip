@@ -163,8 +163,8 @@ void distill_kernel(const Args a) {
   const float c = kLog2e / a.tau, itau = 1.f / a.tau;
   const float weight = a.weight ? a.weight[row] : 1.f;
 
-  // the row's vectors: `head` elements before the first aligned one, this workgroup's vectors [v0, v1), a tail
-  const int head = (int)min((int64_t)((16 - ((uintptr_t)z & 15)) & 15) / (int)sizeof(T), a.V);
+  // the row's vectors: `head` elements before the first that begins a 128-byte line, this workgroup's vectors [v0, v1), a tail
+  const int head = (int)min((int64_t)((128 - ((uintptr_t)z & 127)) & 127) / (int)sizeof(T), a.V);
   const int64_t nv = (a.V - head) / n;
   const int64_t v0 = min((int64_t)part * a.piece, nv), v1 = min(v0 + a.piece, nv);
   const bool first = part == 0, last = part == a.parts - 1;
@@ -199,7 +199,7 @@ void distill_kernel(const Args a) {
     }
   }
   __syncthreads();
-  const int64_t b0 = head + v0 * n - 8;  // column of bit 0, so that a vector's bits lie in one byte
+  const int64_t b0 = head + v0 * n - 64;  // column of bit 0: a vector's bits lie in one byte, the head's before them
   if constexpr (kMode != kFinish) {
     for (int i = tid; i < k; i += kThreads) {
       const int j = s_idx[i];
@@ -257,7 +257,7 @@ void distill_kernel(const Args a) {
     auto vector = [&](int v, uint4 raw) {
       float x[n];
       unpack_vec<kT>(raw, x);
-      const int b = v * n + 8;
+      const int b = v * n + 64;
       const uint32_t mask = (bits[b >> 5] >> (b & 31)) & ((1u << n) - 1);
       if (mask) {
 #pragma unroll
@@ -443,7 +443,7 @@ extern "C" int distill_topk_kl(const void* logits, int64_t type, int64_t ld, int
   const int64_t n = 16 / es, nv = V / n, piece = std::max<int64_t>((nv + parts - 1) / parts, 1);
   MX_CHECK_ARG(piece * n <= kMaxPiece + 8, "distill_topk_kl: too few parts");
   const Args a{logits, ld, V, idx, idx_bytes == 8, ld_idx, t, ld_t, (int)k, tau, lse, weight, loss, grad, ld_grad, (int)parts,
-               0, piece, (int)((piece * n + 8 + 2 * 8) / 32 + 2),  // a piece's columns, 8 before it, head and tail
+               0, piece, (int)((piece * n + 64 + 8) / 32 + 2),  // a piece's columns, 64 before it, the tail
                (float2*)ws, ws ? (float2*)((char*)ws + T * parts * 8) : nullptr};
   const hipStream_t st = (hipStream_t)stream;
   if (type == MXFP4_BF16) launch<MXFP4_BF16>(a, T, (int)stages, st);
