@@ -215,3 +215,36 @@ def test_graph_replays(gpu):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(loss, ref[0]) and torch.equal(g, ref[1]), k
+
+
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("dt,T,V", [(BF, 70, 1), (BF, 70, 5), (BF, 70, 40), (BF, 70, 63), (BF, 70, 64), (BF, 70, 71), (BF, 70, 200),
+                                    (HF, 70, 9000), (F32, 40, 30), (F32, 40, 33), (F32, 40, 5001)])
+def test_rows_that_begin_anywhere_in_a_line(gpu, dt, T, V, rest):
+    """Rows an odd number of elements apart: every place in a 128-byte line is some row's first; the gradient in place, at the
+    same places of other rows' lines, and at other places."""
+    z, idx, t, lse, w = _case(V, T, V, min(V, 6), 1.0, rest, dt)
+    ld = V + (2 if V % 2 else 1)
+    wide = torch.zeros(T, ld, dtype=dt, device=gpu)
+    wide[:, :V] = z.to(gpu)
+    args = idx.to(gpu), t.to(gpu), w.to(gpu), 1.0, None if lse is None else lse.to(gpu)
+    for shift in (0, 16 // wide.element_size(), 1):
+        flat = torch.zeros(T * ld + shift, dtype=dt, device=gpu)
+        out = flat[shift:].view(T, ld)[:, :V]
+        _check(distill.topk_kl_rows(wide[:, :V], *args, out=out), z, idx, t, w, 1.0, lse)
+    got = distill.topk_kl_rows(wide[:, :V], *args, out=wide[:, :V])
+    _check(got, z, idx, t, w, 1.0, lse)
+    assert not wide[:, V:].any()
+
+
+@pytest.mark.parametrize("shift", [0, 1, 8, 37])
+def test_split_rows_that_begin_anywhere_in_a_line(gpu, shift):
+    T, V = 3, 70001
+    z, idx, t, lse, w = _case(3, T, V, 64, 1.0, True, BF)
+    idx[:, :4] = torch.tensor([0, 1, V - 2, V - 1])  # ends of the row, whichever vector or scalar holds them
+    idx[:, 4:] = 2 + idx[:, 4:] % 900 * 77  # some more than once
+    flat = torch.zeros(T * V + 64, dtype=BF, device=gpu)
+    zz = flat[shift:shift + T * V].view(T, V)
+    zz.copy_(z)
+    got = distill.topk_kl_rows(zz, idx.to(gpu), t.to(gpu), w.to(gpu), 1.0, lse.to(gpu))
+    _check(got, z, idx, t, w, 1.0, lse)

@@ -10,6 +10,7 @@ import torch
 import _native
 import distill
 import mxfp4
+import test_gpu_mx4_shapes as shapes
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 HEADER = os.path.join(ROOT, "include", "mxfp4_ops.h")
@@ -117,6 +118,20 @@ def test_plans(lib):
             p = parts(T, V)
             assert 1 <= p <= 256 and -(-V // p) <= 1 << 18
     assert lib.distill_workspace_size(I(3), I(5), I(2)) == 3 * 2 * 8 + 3 * 5 * 8
+
+
+def test_sizes_of_the_shape_tests_take_their_shapes(lib):
+    for table, gated in ((shapes.PLAIN, False), (shapes.GATED, True)):
+        for (shape, act), sizes in table.items():
+            for size in sizes:
+                assert _native.mx4_shape(*size, act, gated) == shape, (size, act, gated)
+                if gated:  # what is saved keeps the launch from the kernel for few rows, and changes nothing else
+                    assert _native.mx4_shape(*size, act, True, saved=True) == ("64x128" if shape == "thin" else shape)
+        assert {a for _, a in table} == {"e4m3", "e2m1"}
+    assert {s for s, _ in shapes.PLAIN} == {"thin", "64x64", "64x128", "128x128", "256x128"}
+    assert {s for s, _ in shapes.GATED} == {"thin", "64x128", "128x128", "256x128"}
+    with pytest.raises(_native.NativeError):
+        _native.mx4_shape(0, 1, 1)
 
 
 def test_cpu_tensors_and_names_are_refused():

@@ -251,6 +251,13 @@ def gemm_shape(M, N, K, kind="plain", cus=256):
     return host().gemm_shape(M, N, K, GEMM_KINDS.index(kind), cus)
 
 
+def mx4_shape(M, N, K, act="e4m3", gated=False, saved=False, cus=256):
+    """The workgroup shape of a 4-bit product of more than 16 rows with weight rows N (gated: N of gate and of up) on a GPU of
+    `cus` CUs; saved: the gated block keeps what its backward needs.  Host code only."""
+    rows = (N + 31) // 32 * 64 if gated else N
+    return host4().shape(M, rows, K, act == "e4m3", gated, not saved, cus)
+
+
 def gemm_nt(a, sa, lda, b, sb, ldb, M, N, K, c, lora=None, alpha=1.0, split=True, layout=0):
     """c[M, N] = bf16(A·Bᵀ) [+ alpha · P·Qᵀ with lora = (P [M, r], Q [N, r])].  layout bit 0 / 1: A / B codes
     MX-tiled; bit 2 (GEMM_WIDE): 8-wave 256 x 256 workgroups, whose tail tiles split along K through the cached

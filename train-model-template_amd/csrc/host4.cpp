@@ -19,6 +19,7 @@
 
 #include "../../include/mxfp4_ops.h"
 #include "../../include/mxfp8_mlp.h"
+#include "mx4_plan.h"
 
 namespace py = pybind11;
 using at::Tensor;
@@ -515,6 +516,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     g_error = e.ptr();
   });
   m.def("abi_version", [] { return (int64_t)MXFP4_OPS_ABI_VERSION; });
+  m.def("shape", [](int64_t M, int64_t rows, int64_t K, bool e4m3, bool gated, bool thin, int64_t cus) {
+    need(M > 0 && rows > 0 && K > 0 && cus > 0 && std::max({M, rows, K, cus}) < (1 << 30), "mx4_shape", "bad size");
+    static const char* const names[] = {"256x128", "128x128", "64x128", "64x64", "thin"};
+    return std::string(names[mx4_shape(M, rows, (K + 127) / 128, e4m3, gated, thin, (int)cus)]);
+  });
   py::class_<Weight, WeightP>(m, "Weight")
       .def(py::init(&make_weight), Free())
       .def_readonly("N", &Weight::N)
