@@ -9,6 +9,7 @@ import math
 import pytest
 import torch
 
+import _native
 import distill
 from oracle import distill as od
 
@@ -248,3 +249,26 @@ def test_split_rows_that_begin_anywhere_in_a_line(gpu, shift):
     zz.copy_(z)
     got = distill.topk_kl_rows(zz, idx.to(gpu), t.to(gpu), w.to(gpu), 1.0, lse.to(gpu))
     _check(got, z, idx, t, w, 1.0, lse)
+
+
+def test_a_buffer_over_the_logits_is_their_own_or_apart(gpu):
+    """In place or beside the logits; a buffer that overlaps them otherwise is refused, and autograd sees the write."""
+    z, idx, t, _, w = _case(2, 5, 40, 3, 1.0, False, BF)
+    args = idx.to(gpu), t.to(gpu), w.to(gpu)
+    buf = torch.zeros(6, 100, dtype=BF, device=gpu)
+    zz = buf[:5, :40]
+    zz.copy_(z)
+    ref = distill.topk_kl_rows(zz, *args)[1]
+    beside = buf[:5, 40:80]
+    assert torch.equal(distill.topk_kl_rows(zz, *args, out=beside)[1], ref)
+    for bad in (buf[1:, :40], buf[:5, 39:79], buf.view(-1)[:200].view(5, 40), buf.view(-1)[99:499].view(5, 80)[:, :40]):
+        with pytest.raises(_native.NativeError, match="overlap"):
+            distill.topk_kl_rows(zz, *args, out=bad)
+    flat = torch.zeros(400, dtype=BF, device=gpu)  # one after the other
+    flat[:200] = z.to(gpu).view(-1)
+    distill.topk_kl_rows(flat[:200].view(5, 40), *args, out=flat[200:].view(5, 40))
+    x = z.to(gpu).requires_grad_(True)
+    y = torch.tanh(x)  # keeps its result
+    distill.topk_kl_rows(y.detach(), *args, out=y.detach())
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.sum().backward()

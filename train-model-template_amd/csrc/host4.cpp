@@ -425,6 +425,18 @@ Tensor row_weight(const Kl& c, const Tensor& w) {
   return w.to(at::kFloat).contiguous();
 }
 
+// Two matrices [T, V] with rows of contiguous columns that are the same memory, row by row, or share none
+bool apart(const Tensor& a, const Tensor& b, int64_t T, int64_t V) {
+  const int64_t es = (int64_t)a.element_size(), row = V * es;  // bytes from here on
+  const int64_t la = T == 1 ? row : a.stride(0) * es, lb = T == 1 ? row : b.stride(0) * es;
+  const int64_t pa = (int64_t)(uintptr_t)a.data_ptr(), pb = (int64_t)(uintptr_t)b.data_ptr();
+  if (!T || (pa == pb && la == lb)) return true;
+  if (pa + (T - 1) * la + row <= pb || pb + (T - 1) * lb + row <= pa) return true;
+  if (la != lb || la == 0) return false;
+  const int64_t d = ((pb - pa) % la + la) % la;  // columns of one buffer's rows beside each other
+  return d >= row && d + row <= la;
+}
+
 std::tuple<Tensor, Tensor> topk_kl_rows(const Tensor& z, const Tensor& idx, const Tensor& t, const OptT& weight, double tau,
                                         const OptT& lse, const OptT& out) {
   const char* what = "topk_kl_rows";
@@ -438,6 +450,8 @@ std::tuple<Tensor, Tensor> topk_kl_rows(const Tensor& z, const Tensor& idx, cons
     need(out->dim() == 2 && out->sizes() == z.sizes() && out->scalar_type() == z.scalar_type() &&
              (out->stride(1) == 1 || c.V == 1) && (c.T <= 1 || out->stride(0) >= c.V),
          what, "the gradient's buffer has the logits' shape and type, contiguous columns and rows that do not overlap");
+    need(apart(z, *out, c.T, c.V), what, "the gradient's buffer is the logits' own or does not overlap them");
+    out->unsafeGetTensorImpl()->bump_version();  // autograd holds no value of it to be the one it saved
     grad = *out;
   } else {
     grad = empty({c.T, c.V}, z.scalar_type(), z);

@@ -8,8 +8,9 @@
 // holds a whole 32-block of token l % 16) and two lane swaps in E4M3 (each block lies in two lanes), so every wave
 // quantizes what it multiplies, from registers, while its weight blocks are under way.
 //
-// thin_kernel does the same for 17 to 64 rows of a quantized operand, which lies in memory as the instruction takes it: up to
-// four 16-row blocks of tokens for each weight block.  Tiles of 64 rows leave most CUs without work there.
+// thin_kernel does the same for 17 to 64 rows of a quantized operand (32 in E4M3), which lies in memory as the instruction
+// takes it: up to four 16-row blocks of tokens for each weight block.  Tiles of 64 rows leave most CUs without work there:
+// mx4_plan.h has both sides' times.  32 x 2048 x 12288 takes 8.5 us in E2M1 and 12.4 in E4M3; every workgroup reads all of x.
 #include "abi_common.h"
 #include "mx4_device.h"
 #include "mx4_plan.h"

@@ -3,12 +3,18 @@
 // h = fn(g) u.
 //
 // A workgroup computes a kBM x kBN tile with kWM x kWN waves, each kMB x kNB blocks of 32 x 32.  Operands come straight
-// from memory into a ring of LDS stages (global_load_lds), one stage a K tile of 128 codes: the 1 KB blocks of the tiled
-// layouts, which are the LDS image already, and the 512-byte scale tiles of that K tile.  A stage is two matrix steps of 64
-// codes; the first reads the second's fragments, the second waits for the next stage, passes the barrier and reads on, so
-// there is one barrier for every 128 codes, and a step's LDS reads and DMAs stand between its matrix instructions.
+// from memory into a ring of LDS stages (global_load_lds) of kKS matrix steps of 64 codes: the 1 KB blocks of the tiled
+// layouts, which are the LDS image already, and the 512-byte scale tiles of the K tile.  A step's LDS reads and DMAs stand
+// between its matrix instructions; the fragments are read a step ahead of their use, or a whole K tile (kDeep) where
+// registers allow.
 // The matrix instruction takes B's fragment first, so a lane's accumulators are one row m and, with B's rows in the PI
 // order, 16 contiguous columns.
+//
+// What bounds it.  Large products: in E4M3 the matrix pipe, busy 60-65% of cycles at a clock that the power limit holds at
+// 1.9 GHz (10752 x 2048 x 12288 205 us, 2.6 PFLOP/s); in E2M1, at 3.5-3.7 PFLOP/s (10752 x 2048 x 6144 73-77 us, x 6144 x 2048
+// 77-82), the pipe is busy 38-44% at 2.0 GHz and no other unit more (LDS 17-20%, reads of 340 cycles, 82% of them from L2):
+// waves wait to issue, and a tile's fill and epilogue are 3 of its 10 us at K = 2048.  Small ones: the chain of a tile's K
+// tiles, 0.10 (E2M1) to 0.15 us (E4M3) each.
 #include <algorithm>
 #include <type_traits>
 
