@@ -171,3 +171,22 @@ def test_gradients_of_another_type_and_refused_types(gpu):
     assert torch.equal(got, x.grad)
     with pytest.raises(_native.NativeError):
         mxfp4.mx4_linear(x.double(), W)
+
+
+def test_enabled_layers_cast_under_autocast_as_linears_do(gpu):
+    m = _model(gpu)
+    mod = m.model.layers[0].mlp
+    mxfp4.enable_mxfp4(m)
+    x = torch.randn(30, 160, generator=torch.Generator().manual_seed(1)).to(gpu).requires_grad_(True)
+    with torch.autocast("cuda", BF):
+        y = mod(x)
+    y.sum().backward()
+    assert y.dtype == BF and x.grad.dtype == torch.float32
+    assert torch.equal(y, mod(x.detach().to(BF)))
+    with pytest.raises(_native.NativeError):
+        mod(x)  # fp32 and no autocast
+    a = workloads.build_attn(128, 128, 64, 8, 8, device=gpu)
+    mxfp4.enable_mxfp4(a)
+    q = a.model.layers[0].self_attn.q_proj.base_layer
+    with torch.autocast("cuda", torch.float16):
+        assert q(torch.randn(3, 128, device=gpu)).dtype == torch.float16

@@ -154,6 +154,12 @@ def _adapter(x, part):
     return None if A is None else ((x @ A.to(x.dtype).t()) @ B.to(x.dtype).t()) * s
 
 
+def _autocast(x):
+    """x as a linear under autocast takes it."""
+    on = x.is_cuda and x.dtype == torch.float32 and torch.is_autocast_enabled("cuda")
+    return x.to(torch.get_autocast_dtype("cuda")) if on else x
+
+
 def mlp(mod, x):
     """down(fn(gate(x)) * up(x)) of a gated MLP that enable_mxfp4 took: one gated block over the gate and up weights with
     their adapters' outputs added before the gate, and one linear."""
@@ -161,6 +167,7 @@ def mlp(mod, x):
     parts = [_lora(getattr(mod, n)) for n in ("gate_proj", "up_proj", "down_proj")]
     if None in parts:
         raise ValueError("mxfp4.mlp: gate, up and down take plain frozen linears or one LoRA adapter without dropout, unmerged")
+    x = _autocast(x)
     g, u = _adapter(x, parts[0]), _adapter(x, parts[1])
     add = None
     if g is not None or u is not None:
@@ -177,7 +184,7 @@ def _linear_forward(self, x):
     W, act = self._mx4
     if W is None:
         raise RuntimeError("this projection is held by its MLP's gated block (mxfp4.enable_mxfp4) and has no call of its own")
-    return mx4_linear(x, W, act=act)
+    return mx4_linear(_autocast(x), W, act=act)
 
 
 def enable_mxfp4(model, act="e4m3"):
