@@ -3,11 +3,12 @@
 // activations' type).
 //
 // What bounds it: memory, 6 bytes read and 2 (E4M3) or 1 (E2M1) written for each column of a row, and 4 more for the addend's
-// gradient: 10752 x 6144 bf16 in E4M3 takes 90 us, 188 with the addend's gradient (5.9 and 4.2 TB/s; part of it comes from the
-// last-level cache).  The saved values lie in the order of the forward epilogue's lanes, which is this kernel's order too:
-// lane l of a wave holds row l % 32 and 16 columns of a 32 x 32 block, a 32-column scale block is two lanes, and every load of
-// the saved values is 1 KB in a row.  One block a wave: four in a row, each asked for while the one before was computed, took
-// 98 and 206 us, and 15.2 where this takes 12.5 at 1000 x 3584, whose waves then waited four times for memory.
+// gradient: 10752 x 6144 bf16 in E4M3 takes 90 us, 158 with the addend's gradient (5.9 and 5.0 TB/s; part of it comes from the
+// last-level cache); in pieces of 16 bytes of a row that gradient took 30 more.  The saved values lie in the order of the
+// forward epilogue's lanes, which is this kernel's order too: lane l of a wave holds row l % 32 and 16 columns of a 32 x 32
+// block, a 32-column scale block is two lanes, and every load of the saved values is 1 KB in a row.  One block a wave: four in
+// a row, each asked for while the one before was computed, took 98 us, and 11.7 where one takes 9.4 at 1000 x 3584, whose
+// waves then waited four times for memory.
 #include "abi_common.h"
 #include "mx4_device.h"
 
