@@ -70,18 +70,32 @@ def _part(m):
 
 # bf16 copies of the LoRA A/B parameters (fp32) and the concatenated S matrix, made once per training step
 # instead of at every call.  The optimizer may update parameters in place without bumping _version, so the
-# step driver calls new_step() at the start of each step (fused_linear.py:55-62).
+# step driver calls new_step() at the start of each step (fused_linear.py:55-62).  Keys name the parameters by id(), which
+# says nothing once they are gone (a later parameter may get the same one), so an entry goes when the first of its
+# sources does: _SOURCES holds weak references to them, whose callbacks run before an id can come back.
 _CAST = {}
+_SOURCES = {}
 
 
 def new_step():
+    _SOURCES.clear()
     _CAST.clear()
 
 
-def _cast(key, make):
+def _cast(key, make, *src):
+    """The step's value under `key`, made on first use.  src: the tensors whose ids the key holds (none where the value
+    itself keeps them alive)."""
     t = _CAST.get(key)
     if t is None:
-        t = _CAST[key] = make()
+        t = make()
+
+        def drop(_):
+            _CAST.pop(key, None)
+            _SOURCES.pop(key, None)
+
+        if src:
+            _SOURCES[key] = [weakref.ref(s, drop) for s in src]
+        _CAST[key] = t
     return t
 
 
@@ -130,6 +144,8 @@ class _Spec:
         self._adapter = {sl.layer: sl for sl in self.adapters}
         self.mx = [i for i, p in enumerate(parts) if _mx(p[0])]
         self.plain = [i for i, p in enumerate(parts) if not _mx(p[0]) and i not in self.thin_ids]
+        # every parameter that the step's forms of the group are made from: those of S, then the adapters' B
+        self.sources = self.s_sources() + [parts[sl.layer][2] for sl in self.adapters]
 
     def adapter(self, i):
         return self._adapter.get(i)
@@ -162,9 +178,9 @@ def _same_buffer(a, b):
     return a.untyped_storage().data_ptr() == b.untyped_storage().data_ptr()
 
 
-def _s_pad(S, key, rp):
+def _s_pad(S, spec, key, rp):
     """S zero-padded to rp rows (cached per step with the S it pads)."""
-    return _cast(key + ("pad", rp), lambda: torch.cat([S, S.new_zeros(rp - S.shape[0], S.shape[1])]))
+    return _cast(key + ("pad", rp), lambda: torch.cat([S, S.new_zeros(rp - S.shape[0], S.shape[1])]), *spec.sources)
 
 
 # The layout of a group's weight forms, kept across steps: the buffer, its views and the pack job table, keyed
@@ -226,7 +242,7 @@ def _group_forms(spec, skey, K, dev):
     builds these with one operation each."""
     def make():
         import _native
-        srcs = spec.s_sources() + [spec.parts[sl.layer][2] for sl in spec.adapters]
+        srcs = spec.sources
         sig = (K, dev, tuple((sl.col, sl.width) for sl in spec.adapters + spec.thin),
                tuple(spec.parts[i][0].out_features for i in spec.mx),
                tuple((t.data_ptr(), tuple(t.shape), tuple(t.stride()), t.dtype) for t in srcs))
@@ -243,7 +259,7 @@ def _group_forms(spec, skey, K, dev):
             plan = _PLANS[sig] = (forms, _native.pack_table(jobs))
         _native.pack_run(plan[1], like=plan[0].S_pad)
         return plan[0]
-    return _cast(skey + ("forms",), make)
+    return _cast(skey + ("forms",), make, *spec.sources)
 
 
 def _packable(spec, x2, dt):
@@ -254,15 +270,15 @@ def _packable(spec, x2, dt):
             and all(spec.parts[sl.layer][2].dtype in (torch.float32, torch.bfloat16) for sl in spec.adapters))
 
 
-def _thin_product(x2, S, skey, width, dt, S_pad=None):
+def _thin_product(x2, S, spec, skey, dt, S_pad=None):
     """bf16(x2 · Sᵀ): one read of x2 on the library's rank-r kernel (S zero-padded to 16/32/64 rows, so xS has
-    zero columns past `width`) when it applies, else a torch GEMM."""
-    if not _native_ok(x2, dt, width):
+    zero columns past the group's width) when it applies, else a torch GEMM."""
+    if not _native_ok(x2, dt, spec.width):
         return x2 @ S.t()
     import _native
-    rp = _rp(width)
+    rp = _rp(spec.width)
     xS = torch.empty((x2.shape[0], rp), dtype=dt, device=x2.device)
-    _native.lora_nt(x2, _s_pad(S, skey, rp) if S_pad is None else S_pad, xS)
+    _native.lora_nt(x2, _s_pad(S, spec, skey, rp) if S_pad is None else S_pad, xS)
     return xS
 
 
@@ -314,7 +330,7 @@ def _fwd_merged(spec, Bs, xS, codes, T, dt, skey):
     if forms is not None and forms.Q is not None and forms.rp == rp:
         Q = forms.Q
     else:
-        Q = _cast(skey + ("qcat", tuple(spec.mx), rp), block_diagonal_b)
+        Q = _cast(skey + ("qcat", tuple(spec.mx), rp), block_diagonal_b, *spec.sources)
     # every layer with an adapter of one width: each output tile takes the rank-width window of xS and Q at its
     # layer's own columns (the rest of its Q row is zero) instead of all rp columns
     ranks = {sl.width for sl in slots if sl is not None}
@@ -375,7 +391,7 @@ class _Group(torch.autograd.Function):
             x2 = x2.to(dt).contiguous()
         spec = _Spec(parts)
         src = spec.s_sources()
-        skey = (tuple(id(t) for t in src), dt)
+        skey = (tuple(id(t) for t in spec.sources), dt)
         codes = None
         forms = None
         if _packable(spec, x2, dt):
@@ -389,12 +405,12 @@ class _Group(torch.autograd.Function):
                 q, sc, xS, _ = mxfp8.mx_quant_lora(x2, forms.S_pad, out_t=False)
                 codes = (q, sc) if need_out else None
             else:
-                xS = _thin_product(x2, S, skey, spec.width, dt, S_pad=forms.S_pad)
+                xS = _thin_product(x2, S, spec, skey, dt, S_pad=forms.S_pad)
         else:
-            Bs = [_cast((id(parts[sl.layer][2]), dt), lambda B=parts[sl.layer][2]: B.detach().to(dt))
-                  for sl in spec.adapters]
-            S = _cast(skey, lambda: torch.cat([t.detach().to(dt) for t in src])) if src else None
-            xS = _thin_product(x2, S, skey, spec.width, dt) if src else None
+            Bs = [_cast((id(B), dt), lambda B=B: B.detach().to(dt), B)
+                  for B in (parts[sl.layer][2] for sl in spec.adapters)]
+            S = _cast(skey, lambda: torch.cat([t.detach().to(dt) for t in src]), *spec.sources) if src else None
+            xS = _thin_product(x2, S, spec, skey, dt) if src else None
         if need_out:
             outs = _forward_outputs(spec, x2, xS, Bs, skey, defer, dt, codes)
         else:  # only the graph for backward is needed (x2, xS saved); nobody reads the outputs

@@ -198,7 +198,8 @@ def _prep(Ag, Bg, Au, Bu, Ad, Bd, dt):
     def make():
         return types.SimpleNamespace(**dict(zip(_FORMS, _native.host().mlp_forms(
             (Ag, Bg, Au, Bu, Ad, Bd), _native.stream_of(Ag, "mxfp8_lora_prep")))))
-    return _cast((("lora_prep", id(Ag), id(Au), id(Bg), id(Bu), id(Ad), id(Bd)), dt), make)
+    src = (Ag, Au, Bg, Bu, Ad, Bd)
+    return _cast((("lora_prep", *map(id, src)), dt), make, *src)
 
 
 def _forms_key(S, bg, bu, ad, bd, dt):
