@@ -355,9 +355,16 @@ def lora_prep(Ag, Au, Bg, Bu, Ad, Bd, out):
          *[_p(out[k]) for k in ("S", "ST", "bg", "bu", "bgT", "buT", "ad", "adT", "bd", "bdT")], like=Ag)
 
 
+def _check_w(what, w, K):
+    """w [*, K] bf16 without gaps, as the kernels read it by x's width."""
+    if w.dim() != 2 or w.shape[1] != K or not w.is_contiguous() or w.dtype != torch.bfloat16:
+        raise NativeError(f"{what}: w of {tuple(w.shape)} {w.dtype}, [*, {K}] contiguous bf16 expected")
+
+
 def lora_nt(x, w, out, scale=1.0, outT=None):
     """out[t, ρ] = bf16(x[t] · w[ρ]) (then · scale); outT [rp, Tpad] optional (zero-padded transposed copy)."""
     T, K = x.shape
+    _check_w("lora_nt", w, K)
     call("mxfp8_lora_nt", _p(x), T, K, x.stride(0), _p(w), w.shape[0], float(scale), _p(out), _p(outT),
          outT.shape[1] if outT is not None else 0, like=x)
 
@@ -365,6 +372,7 @@ def lora_nt(x, w, out, scale=1.0, outT=None):
 def quant_lora(x, q, s, w, out, scale=1.0, outT=None):
     """mxfp8.mx_quant_tiled(x) into (q, s) and lora_nt(x, w, out, scale, outT) from one read of x."""
     T, K = x.shape
+    _check_w("quant_lora", w, K)
     call("mxfp8_quant_lora", _p(x), T, K, x.stride(0), _p(q), _p(s), _p(w), w.shape[0], float(scale), _p(out),
          _p(outT), -(-T // 128) * 128, like=x)
 
@@ -373,6 +381,7 @@ def quant_lora_tp(x, q, s, w, out, tx, tout, scale=1.0, outT=None):
     """quant_lora(x, q, s, w, out, scale, outT) and, in the same launch, tout [C, Tpad] = txᵀ zero-padded
     (transpose_pad of tx [T, C])."""
     T, K = x.shape
+    _check_w("quant_lora_tp", w, K)
     call("mxfp8_quant_lora_tp", _p(x), T, K, x.stride(0), _p(q), _p(s), _p(w), w.shape[0], float(scale), _p(out),
          _p(outT), -(-T // 128) * 128, _p(tx), tx.stride(0), tx.shape[1], _p(tout), like=x)
 

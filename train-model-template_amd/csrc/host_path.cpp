@@ -77,6 +77,20 @@ struct Arena {
   float* f(int64_t off) const { return static_cast<float*>(at(off)); }
 };
 
+// The kernels read w and the rank-r operands by the sizes of x and of the product: other sizes would be read past.
+// w of x . w^T, [.., K] bf16 rows without gaps
+void check_w(const char* what, const Tensor& w, int64_t K) {
+  TORCH_CHECK(w.dim() == 2 && w.size(1) == K && w.is_contiguous() && w.scalar_type() == kBF, what, ": w of ", w.sizes(), " ",
+              w.scalar_type(), ", [*, ", K, "] contiguous bf16 expected");
+}
+// P [M, >= r] and Q [N, >= r] of a product's rank-r epilogue
+void check_lora(const char* what, const OptT& P, const OptT& Q, int64_t M, int64_t N, int64_t r) {
+  if (!P) return;
+  TORCH_CHECK(Q && P->dim() == 2 && Q->dim() == 2 && P->size(0) >= M && Q->size(0) >= N && P->size(1) >= r &&
+                  Q->size(1) >= r && P->scalar_type() == kBF && Q->scalar_type() == kBF,
+              what, ": rank-", r, " operands of other sizes than the product's ", M, " x ", N);
+}
+
 // ------------------------------------------------------------------ single calls
 std::tuple<Tensor, Tensor> quant_rows(const Tensor& x, int64_t stream) {
   gpu(x, "mxfp8_quant_rows");
@@ -96,6 +110,7 @@ std::tuple<Tensor, Tensor> quant_tiled(const Tensor& x, int64_t stream) {
 
 std::tuple<Tensor, Tensor, Tensor, OptT> quant_lora(const Tensor& x, const Tensor& w, double scale, bool out_t,
                                                     int64_t stream) {
+  check_w("quant_lora", w, x.size(1));
   gpu(x, "mxfp8_quant_lora");
   const int64_t R = x.size(0), K = x.size(1), rp = w.size(0), tpad = cdiv(R, 128) * 128;
   Tensor q = empty({tiled_rows(R), K}, kF8, x), s = empty({scale_numel(R, K)}, kE8, x), out = empty({R, rp}, kBF, x);
@@ -110,6 +125,7 @@ std::tuple<Tensor, Tensor, Tensor, OptT> quant_lora(const Tensor& x, const Tenso
 // mxfp8.mx_mm for the shapes without a workspace (every layout but the explicit 8-wave one)
 Tensor gemm(const Tensor& q, const Tensor& s, const Tensor& w, const Tensor& ws, const OptT& out_, const OptT& P,
             const OptT& Q, double alpha, int64_t layout, int64_t M, int64_t stream) {
+  check_lora("gemm", P, Q, M, w.size(0), P ? P->size(1) : 0);
   gpu(q, "mxfp8_gemm_nt");
   const int64_t N = w.size(0), K = q.size(1);
   Tensor out = out_ ? *out_ : empty({layout & MXFP8_GEMM_C_FT ? ft_rows(M) : M, N}, kBF, q);
@@ -124,6 +140,7 @@ Tensor gemm(const Tensor& q, const Tensor& s, const Tensor& w, const Tensor& ws,
 std::vector<Tensor> gemm_seg(const Tensor& q, const Tensor& s, const Tensor& w, const Tensor& ws,
                              const std::vector<int64_t>& widths, const OptT& P, const OptT& Q, double alpha,
                              int64_t layout, int64_t M, const std::vector<int64_t>& rcols, int64_t r, int64_t stream) {
+  check_lora("gemm_seg", P, Q, M, w.size(0), rcols.empty() ? P ? P->size(1) : 0 : *std::max_element(rcols.begin(), rcols.end()) + r);
   gpu(q, "mxfp8_gemm_nt_seg");
   const int64_t N = w.size(0), K = q.size(1), n = (int64_t)widths.size();
   TORCH_CHECK(n >= 1 && n <= 4, "gemm_seg: 1 to 4 outputs");
@@ -165,6 +182,7 @@ using TnJob = std::tuple<Tensor, Tensor, Tensor, double, bool>;  // x, p, out, s
 Tensor gemm_tn(const Tensor& q, const Tensor& s, const Tensor& w, const Tensor& ws, const Tensor& P, const Tensor& Q,
                double alpha, int64_t layout, int64_t M, const std::vector<TnJob>& jobs, const Tensor& part,
                int64_t stream) {
+  check_lora("gemm_tn", P, Q, M, w.size(0), P.size(1));
   gpu(q, "mxfp8_gemm_nt_tn");
   const int64_t N = w.size(0), K = q.size(1), n = (int64_t)jobs.size();
   TORCH_CHECK(n >= 1 && n <= MXFP8_LORA_TN_MAX_JOBS, "gemm_tn: 1 to ", MXFP8_LORA_TN_MAX_JOBS, " reductions");
@@ -287,6 +305,7 @@ std::tuple<Tensor, Tensor, Tensor> mlp_forward(const Tensor& x, const Tensor& S,
   const int64_t T = x.size(0), K = x.size(1), R = ad.size(0), N = ad.size(1);
   check_cols("mlp_forward: gate|up weight", wf, K);
   check_cols("mlp_forward: down weight", wd, N);
+  check_w("mlp_forward", S, K);
   gpu(x, "mxfp8_gemm_swiglu_fwd");
   Tensor xs = empty({T, 2 * R}, kBF, x), gu = empty({ft_rows(T), 2 * N}, kBF, x), y;
   const int64_t parts = 2 * N / 128;
@@ -332,6 +351,7 @@ std::tuple<Tensor, Tensor> mlp_graph(const Tensor& x, const Tensor& S, const Ten
                                      int64_t stream) {
   const int64_t T = x.size(0), K = x.size(1), rp = S.size(0);
   check_cols("mlp_graph: gate|up weight", w, K);
+  check_w("mlp_graph", S, K);
   gpu(x, "mxfp8_gemm_nt");
   Tensor xs = empty({T, rp}, kBF, x), gu = empty({ft_rows(T), 2 * N}, kBF, x);
   Arena a;
