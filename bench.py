@@ -340,6 +340,7 @@ def _unfused_mlp(T, K, N, r, dev, steps=10):
     import torch
 
     import _native
+    import fused_linear
     import fused_mlp
     import mxfp8
     import shared_prefix
@@ -363,6 +364,7 @@ def _unfused_mlp(T, K, N, r, dev, steps=10):
     params = [p for p in mlp.parameters() if p.requires_grad]
 
     def step():
+        fused_linear.new_step()
         y = shared_prefix._mlp(mlp, x)
         y.backward(dy)
         for p in params:
