@@ -13,7 +13,8 @@ follows the same columns.  On that layout:
     concatenated Wᵀ, with dS·S in its epilogue; other groups take the per-layer backward;
   - o_proj / out_proj may return a Deferred output (LoRA not yet added) that residual_add adds inside the residual
     kernel (mxfp8.res_lora).
-Layers that cannot be grouped (trainable base weights, DoRA, dropout > 0, several adapters) are called one by one.
+Layers that cannot be grouped (trainable base weights, DoRA, dropout > 0, several adapters, weights in MXFP4) are called
+one by one.
 `_part`, `_cast` / `new_step` and `STATS` are also what the fused MLP path reads.
 """
 import dataclasses
@@ -48,7 +49,14 @@ def _attr(m, name, *default):
 
 def _part(m):
     """(base Linear, A, B, scaling) of a PEFT LoRA Linear; (m, None, None, 1.0) for a plain frozen Linear;
-    None if the layer cannot be grouped (fused_linear.py:30-48)."""
+    None if the layer cannot be grouped (fused_linear.py:30-48).  A linear that mxfp4.enable_mxfp4 took holds no weight
+    here: it is called by itself."""
+    part = _adapted(m)
+    return None if part is None or "_mx4" in part[0].__dict__ else part
+
+
+def _adapted(m):
+    """_part, whatever form the base weight is in."""
     base = _attr(m, "base_layer", None)
     if base is None:
         if type(m) is nn.Linear and _attr(m, "bias") is None and not _attr(m, "weight").requires_grad:

@@ -22,7 +22,7 @@ from torch import nn
 
 import _native
 import mxfp8
-from fused_linear import _part
+from fused_linear import _adapted
 
 E2M1, E4M3 = 4, 8
 _FMT = {"e2m1": E2M1, "e4m3": E4M3}
@@ -142,8 +142,8 @@ def _gate_name(mlp):
 
 
 def _lora(proj):
-    """_part, and the base layer alone where the adapters are switched off for a while."""
-    part = _part(proj)
+    """fused_linear._adapted, and the base layer alone where the adapters are switched off for a while."""
+    part = _adapted(proj)
     off = part is None and getattr(proj, "disable_adapters", False) and not proj.merged
     return (proj.base_layer, None, None, 1.0) if off else part
 

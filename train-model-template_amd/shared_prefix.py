@@ -47,8 +47,9 @@ def _SWIGLU(g, u):
 def _mlp(mlp, x, need_out=True):
     """down(silu(gate(x)) * up(x)) as a Qwen3.5 MLP (shared_prefix.py:179-197): the fused MXFP8 MLP when gate/up
     are paired by mxfp8.enable_mxfp8 and fused_mlp.mlp takes the shapes, else gate/up as one group_linear, SwiGLU,
-    and down as a group_linear.  need_out=False: the down GEMM's output is not computed (see group_linear)."""
-    if type(mlp.act_fn).__name__ not in ("SiLU", "SiLUActivation"):
+    and down as a group_linear.  need_out=False: the down GEMM's output is not computed (see group_linear).  An MLP
+    with another gate function, or one that mxfp4.enable_mxfp4 took whole, is called as it is."""
+    if "_mx4_gated" in mlp.__dict__ or type(mlp.act_fn).__name__ not in ("SiLU", "SiLUActivation"):
         STATS["mlp gọi thẳng"] = STATS.get("mlp gọi thẳng", 0) + 1
         return mlp(x)
     if getattr(getattr(mlp.gate_proj, "base_layer", mlp.gate_proj), "_mx_gu", None) is not None:
