@@ -359,6 +359,8 @@ __device__ __forceinline__ void store_block(typename Elem<kT>::T* p, int64_t ld,
 // gelu(g) = g s(2 c (g + a g^3)) with c = sqrt(2 / pi), a = 0.044715 (0.5 (1 + tanh t) = sigmoid(2 t)), so
 // gelu' = s + g s (1 - s) 2 c (1 + 3 a g^2).  Both with the hardware exp2 and reciprocal, 1 ulp each.
 // 1 - s is off by 2^-24 where s is near 1, which g (1 - s) + 1 takes as g 2^-24.
+// gelu' takes its polynomial at g held to +-16, past which s is 0 or 1 in 32 bits (t is +-317 there) and gelu' with it: the
+// powers of a larger g would pass 32 bits and give inf * 0.
 template <int kFn>
 __device__ __forceinline__ float gate_fn(float g) {
   if constexpr (kFn == MXFP4_SILU) {
@@ -375,10 +377,10 @@ __device__ __forceinline__ float gate_fn(float g, float& df) {
     df = s * __builtin_fmaf(g, 1.f - s, 1.f);
     return g * s;
   } else {
-    const float q = 0.044715f * g * g;
-    const float t = 1.5957691216057308f * g * (1.f + q);
+    const float k = __builtin_amdgcn_fmed3f(g, -16.f, 16.f), q = 0.044715f * k * k;
+    const float t = 1.5957691216057308f * g * (1.f + q);  // of g itself: NaN stays
     const float s = fast_sigmoid(t);
-    df = s * __builtin_fmaf(g * 1.5957691216057308f * __builtin_fmaf(3.f, q, 1.f), 1.f - s, 1.f);
+    df = s * __builtin_fmaf(k * 1.5957691216057308f * __builtin_fmaf(3.f, q, 1.f), 1.f - s, 1.f);
     return g * s;
   }
 }
