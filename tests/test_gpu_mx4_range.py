@@ -47,3 +47,36 @@ def test_a_nan_gate_stays_nan(gpu):
         h.sum().backward()
         bad = torch.isnan(a.grad)
         assert torch.isnan(h[1, 5]) and bad[1, 5] and bad[1, N + 5] and int(bad.sum()) == 2
+
+
+@pytest.mark.parametrize("fmt", ["e2m1", "e4m3"])
+@pytest.mark.parametrize("dt", [BF, torch.float32])
+def test_blocks_at_the_least_scale(gpu, dt, fmt):
+    """Blocks around the largest value times 2^-127 and far below, denormals among them: the scale is 2^-127 at the least
+    and codes are of v 2^127, in both axes and in the kernels that quantize their rows themselves."""
+    g = torch.Generator().manual_seed(2)
+    x = torch.zeros(40, 256, dtype=torch.float64)
+    for i in range(40):  # from 2^-110 down to the least denormals
+        x[i] = torch.randn(256, generator=g, dtype=torch.float64) * 2.0 ** (-110 - i)
+    x[39, :32] = 448 * 2.0 ** -127
+    x[38, :32] = 448 * 2.0 ** -127 * torch.linspace(0, 1, 32, dtype=torch.float64)
+    x[37, :32] = 6 * 2.0 ** -127 * torch.linspace(-1, 1, 32, dtype=torch.float64)
+    x = x.float().to(dt)
+    m, mt = mxfp4.mx4_quant(x.to(gpu), fmt=fmt, both=True)
+    for got, ref in ((m, x), (mt, x.t())):
+        v = mxfp4.mx4_dequant(got).double().cpu()
+        assert torch.equal(v, mx4.values(ref, fmt)), int((v != mx4.values(ref, fmt)).sum())
+
+
+def test_products_of_rows_at_the_least_scale(gpu):
+    """Rows of 2^-120 against weights of 2^100: what the quantizer keeps of them comes out of the product in both formats,
+    of few rows and of many."""
+    g = torch.Generator().manual_seed(3)
+    x = (torch.randn(40, 256, generator=g) * 2.0 ** -121).to(BF)
+    w = (torch.randn(64, 256, generator=g) * 2.0 ** 100).to(BF)
+    W = mxfp4.Weight(w.to(gpu))
+    for act in ("e4m3", "e2m1"):
+        ref, mag = mx4.linear(x, w, act)
+        for rows in (40, 5):
+            y = mxfp4.mx4_linear(x[:rows].to(gpu), W, act=act).double().cpu()
+            assert ((y - ref[:rows]).abs() <= 2.0 ** -8 * ref[:rows].abs() + 2.0 ** -12 * mag[:rows]).all()

@@ -40,13 +40,8 @@ __device__ __forceinline__ uint32_t block_exponent(uint32_t amax_b) {
   return (uint32_t)e;
 }
 
-// 2^(e - 127) as a float; e = 0 gives the denormal 2^-127 (E4M3 scales by 1 there, as the 8-bit quantizer does: every
-// code of such a block is 0 either way)
-template <int kFmt>
-__device__ __forceinline__ float block_scale(uint32_t e) {
-  if constexpr (kFmt == MXFP4_E4M3) return __uint_as_float(e == 0u ? 0x3f800000u : e << 23);
-  return __uint_as_float(e == 0u ? 1u << 22 : e << 23);
-}
+// 2^(e - 127) as a float; e = 0 gives the denormal 2^-127
+__device__ __forceinline__ float block_scale(uint32_t e) { return __uint_as_float(e == 0u ? 1u << 22 : e << 23); }
 
 // Codes of eight values that share the block exponent e: E2M1 in r[0], E4M3 in r[0], r[1].
 // Values of finite blocks are within the format's range by the choice of e.  Blocks with an infinity clamp, blocks with a
@@ -55,7 +50,7 @@ template <int kFmt>
 __device__ __forceinline__ void encode8(const float* v, uint32_t e, uint32_t* r) {
   constexpr float kMax = kFmt == MXFP4_E4M3 ? 448.f : 6.f;
   float w[8];
-  float sc = block_scale<kFmt>(e);
+  float sc = block_scale(e);
 #pragma unroll
   for (int i = 0; i < 8; ++i) w[i] = v[i];
   if (__builtin_expect(__builtin_amdgcn_ballot_w64(e >= 254u) != 0, 0)) {
@@ -149,7 +144,7 @@ __device__ __forceinline__ void encode_group(const Group<kT>& g, uint32_t e, uin
       encode8<kFmt>(v, e, r);
       return;
     }
-    const float sc = block_scale<kFmt>(e);
+    const float sc = block_scale(e);
     const uint32_t u[4] = {g.w.x, g.w.y, g.w.z, g.w.w};
     if constexpr (kFmt == MXFP4_E4M3) {
 #pragma unroll
