@@ -212,6 +212,10 @@ using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
 
 bool records(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+// The nodes below know the backward pass alone: the tangent of a dual tensor would be lost
+void no_tangent(const Tensor& t, const char* what) {
+  need(!t._fw_grad(0).defined(), what, "no forward-mode derivative");
+}
 void once(const char* what) {
   need(!at::GradMode::is_enabled(), what, "the backward pass has no derivative of its own (create_graph)");
 }
@@ -231,6 +235,7 @@ struct LinearNode : Node {
 };
 
 Tensor linear(const WeightP& w, const Tensor& x, int64_t fmt, bool forward) {
+  no_tangent(x, "mx4_linear");
   if (!records(x))
     return forward ? product(x, w->q, w->s, w->N, w->K, fmt) : product(x, w->qt, w->st, w->K, w->N, fmt);
   if (!w->qt.defined())
@@ -349,6 +354,8 @@ struct GatedNode : Node {
 
 Tensor gated(const GatedP& w, const Tensor& x, const OptT& add_, int64_t fn, int64_t fmt) {
   const char* what = "mx4_gated";
+  no_tangent(x, what);
+  if (add_) no_tangent(*add_, what);
   gpu(x, what);
   same(x, w->q, what);
   half_type(x, what);
@@ -440,6 +447,7 @@ bool apart(const Tensor& a, const Tensor& b, int64_t T, int64_t V) {
 std::tuple<Tensor, Tensor> topk_kl_rows(const Tensor& z, const Tensor& idx, const Tensor& t, const OptT& weight, double tau,
                                         const OptT& lse, const OptT& out) {
   const char* what = "topk_kl_rows";
+  no_tangent(z, what);
   gpu(z, what);
   const Scope sc(z);
   const Kl c = kl_call(z, idx, t, tau, lse);
@@ -484,6 +492,7 @@ struct KlNode : Node {
 };
 
 Tensor topk_kl(const Tensor& z, const Tensor& idx, const Tensor& t, double tau, const OptT& lse) {
+  no_tangent(z, "topk_kl");
   gpu(z, "topk_kl");
   const bool rec = records(z);
   Tensor loss, ws;
