@@ -155,8 +155,8 @@ def _adapter(x, part):
 
 
 def _autocast(x):
-    """x as a linear under autocast takes it."""
-    on = x.is_cuda and x.dtype == torch.float32 and torch.is_autocast_enabled("cuda")
+    """x as a linear under autocast takes it: every floating type but float64 in autocast's."""
+    on = x.is_cuda and x.is_floating_point() and x.dtype != torch.float64 and torch.is_autocast_enabled("cuda")
     return x.to(torch.get_autocast_dtype("cuda")) if on else x
 
 
