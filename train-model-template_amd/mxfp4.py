@@ -212,7 +212,7 @@ def enable_mxfp4(model, act="e4m3"):
     for lin in found.values():
         w = lin.weight.data
         lin._mx4 = (held[id(lin)] if id(lin) in held else Weight(w), act)
-        lin._bf16_cpu = w.to("cpu", copy=True)
+        lin._mx4_cpu = w.to("cpu", copy=True)
         lin.weight.data = torch.empty((0,), dtype=w.dtype, device=w.device)
         lin.forward = types.MethodType(_linear_forward, lin)
     torch.cuda.empty_cache()
@@ -225,6 +225,6 @@ def disable_mxfp4(model):
         if "_mx4_gated" in mod.__dict__:
             del mod._mx4_gated, mod.forward
         if "_mx4" in mod.__dict__:
-            mod.weight.data = mod._bf16_cpu.to(mod.weight.device)
-            del mod._mx4, mod._bf16_cpu, mod.forward
+            mod.weight.data = mod._mx4_cpu.to(mod.weight.device)
+            del mod._mx4, mod._mx4_cpu, mod.forward
     torch.cuda.empty_cache()

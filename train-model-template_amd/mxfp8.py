@@ -716,6 +716,8 @@ def enable_mxfp8(model):
     (mxfp8.py:452-498).  Both axes of each weight come from one read (quant_both).  Returns the linear count."""
     found, owners = [], {}
     for name, lin in _base_linears(model):
+        if "_mx4" in lin.__dict__:
+            raise ValueError(f"enable_mxfp8: {name} holds its weight in MXFP4 (mxfp4.disable_mxfp4 puts it back)")
         assert lin.bias is None
         assert lin.weight.is_cuda and lin.weight.shape[0] % 128 == 0 and lin.weight.shape[1] % 128 == 0, \
             lin.weight.shape
