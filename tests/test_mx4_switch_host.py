@@ -1,5 +1,7 @@
 """enable_mxfp4 and disable_mxfp4 beside the 8-bit switches, on stand-ins of the quantized weights (the quantizer runs on the
 GPU alone): each pair undoes its own work only, and a call that fails leaves the model as it was."""
+import types
+
 import pytest
 import torch
 
@@ -62,3 +64,17 @@ def test_the_four_bit_switches_leave_eight_bit_layers_alone(model):
         mxfp4.enable_mxfp4(model)
     mxfp4.disable_mxfp4(model)
     assert _same(_state(model), on)
+
+
+def test_forwards_patched_before_come_back(model):
+    mlp = model.model.layers[0].mlp
+    lin = model.model.layers[1].mlp.down_proj.base_layer
+    calls = []
+    mlp.forward = types.MethodType(lambda self, x: calls.append("mlp") or x, mlp)
+    lin.forward = types.MethodType(lambda self, x: calls.append("lin") or x, lin)
+    mxfp4.enable_mxfp4(model)
+    assert mlp.forward.__func__ is mxfp4.mlp and lin.forward.__func__ is mxfp4._linear_forward
+    mxfp4.disable_mxfp4(model)
+    mlp(1)
+    lin(1)
+    assert calls == ["mlp", "lin"]

@@ -187,10 +187,24 @@ def _linear_forward(self, x):
     return mx4_linear(_autocast(x), W, act=act)
 
 
+def _patch(mod, forward):
+    """Route mod's calls through `forward`; what its own `forward` attribute was, if it had one, waits in _mx4_forward."""
+    mod._mx4_forward = mod.__dict__.get("forward")
+    mod.forward = types.MethodType(forward, mod)
+
+
+def _unpatch(mod):
+    own = mod.__dict__.pop("_mx4_forward")
+    del mod.forward
+    if own is not None:
+        mod.forward = own
+
+
 def enable_mxfp4(model, act="e4m3"):
     """Quantize every frozen base linear of the decoder layers (those of mxfp8.enable_mxfp8: any shape here, no bias) to
     MXFP4 along both axes, move the weights to host memory and route the layers' forward through mx4_linear.  An MLP with
-    gate_proj, up_proj, down_proj and a SiLU or tanh-GELU act_fn runs as `mlp` instead, if its adapters let it.  LoRA wrappers
+    gate_proj, up_proj, down_proj and a SiLU or tanh-GELU act_fn runs as `mlp` instead, if its adapters let it: hooks on the
+    MLP run, hooks on its three projections do not, and gate_proj and up_proj cannot be called by themselves.  LoRA wrappers
     keep working: their base layer is what changes.  Returns the number of linears."""
     _fmt(act)  # refuses an unknown name before anything is touched
     found = {id(lin): lin for _, lin in mxfp8._base_linears(model)}
@@ -207,14 +221,14 @@ def enable_mxfp4(model, act="e4m3"):
                 and base[0].weight.dtype == base[1].weight.dtype:
             G, D = GatedWeight(base[0].weight, base[1].weight), Weight(base[2].weight)
             mod._mx4_gated = (G, D, _gate_name(mod), act)
-            mod.forward = types.MethodType(mlp, mod)
+            _patch(mod, mlp)
             held.update({id(base[0]): None, id(base[1]): None, id(base[2]): D})
     for lin in found.values():
         w = lin.weight.data
         lin._mx4 = (held[id(lin)] if id(lin) in held else Weight(w), act)
         lin._mx4_cpu = w.to("cpu", copy=True)
         lin.weight.data = torch.empty((0,), dtype=w.dtype, device=w.device)
-        lin.forward = types.MethodType(_linear_forward, lin)
+        _patch(lin, _linear_forward)
     torch.cuda.empty_cache()
     return len(found)
 
@@ -223,8 +237,10 @@ def disable_mxfp4(model):
     """Put the weights back on their device and take the 4-bit copies and the patched forwards away."""
     for mod in model.modules():
         if "_mx4_gated" in mod.__dict__:
-            del mod._mx4_gated, mod.forward
+            del mod._mx4_gated
+            _unpatch(mod)
         if "_mx4" in mod.__dict__:
             mod.weight.data = mod._mx4_cpu.to(mod.weight.device)
-            del mod._mx4, mod._mx4_cpu, mod.forward
+            del mod._mx4, mod._mx4_cpu
+            _unpatch(mod)
     torch.cuda.empty_cache()
