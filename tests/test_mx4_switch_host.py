@@ -78,3 +78,23 @@ def test_forwards_patched_before_come_back(model):
     mlp(1)
     lin(1)
     assert calls == ["mlp", "lin"]
+
+
+@pytest.mark.parametrize("fail_at", [0, 1, 2, 3])
+def test_a_call_that_fails_leaves_the_model_as_it_was(model, monkeypatch, fail_at):
+    """Two MLPs are taken whole; without their act_fn, six linears one by one."""
+    if fail_at >= 2:
+        for layer in model.model.layers:
+            layer.mlp.act_fn = torch.nn.ReLU()
+    before, made = _state(model), []
+
+    def weight(*w):
+        if len(made) == fail_at:
+            raise MemoryError
+        made.append(1)
+        return _Weight(*w)
+
+    monkeypatch.setattr(mxfp4, "Weight", weight)
+    with pytest.raises(MemoryError):
+        mxfp4.enable_mxfp4(model)
+    assert _same(_state(model), before)

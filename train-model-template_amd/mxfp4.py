@@ -205,12 +205,23 @@ def enable_mxfp4(model, act="e4m3"):
     MXFP4 along both axes, move the weights to host memory and route the layers' forward through mx4_linear.  An MLP with
     gate_proj, up_proj, down_proj and a SiLU or tanh-GELU act_fn runs as `mlp` instead, if its adapters let it: hooks on the
     MLP run, hooks on its three projections do not, and gate_proj and up_proj cannot be called by themselves.  LoRA wrappers
-    keep working: their base layer is what changes.  Returns the number of linears."""
+    keep working: their base layer is what changes.  A call that fails leaves the model as it was.  Returns the number of
+    linears."""
     _fmt(act)  # refuses an unknown name before anything is touched
     found = {id(lin): lin for _, lin in mxfp8._base_linears(model)}
     for lin in found.values():
         if lin.bias is not None or mxfp8.is_mx(lin) or "_mx4" in lin.__dict__:
             raise ValueError("enable_mxfp4: linears without bias that are not quantized yet")
+    try:
+        _enable(model, found, act)
+    except BaseException:
+        disable_mxfp4(model)
+        raise
+    torch.cuda.empty_cache()
+    return len(found)
+
+
+def _enable(model, found, act):
     held = {}
     for mod in model.modules():
         projs = [getattr(mod, n, None) for n in ("gate_proj", "up_proj", "down_proj")]
@@ -225,12 +236,10 @@ def enable_mxfp4(model, act="e4m3"):
             held.update({id(base[0]): None, id(base[1]): None, id(base[2]): D})
     for lin in found.values():
         w = lin.weight.data
-        lin._mx4 = (held[id(lin)] if id(lin) in held else Weight(w), act)
-        lin._mx4_cpu = w.to("cpu", copy=True)
+        W, cpu = held[id(lin)] if id(lin) in held else Weight(w), w.to("cpu", copy=True)
+        lin._mx4, lin._mx4_cpu = (W, act), cpu
         lin.weight.data = torch.empty((0,), dtype=w.dtype, device=w.device)
         _patch(lin, _linear_forward)
-    torch.cuda.empty_cache()
-    return len(found)
 
 
 def disable_mxfp4(model):
