@@ -46,7 +46,7 @@ struct Args {
   int64_t piece;   // vectors of a piece
   int bit_words;   // words of LDS for the bits
   float2* stats;   // [T][parts] running maximum and sum of the piece
-  float2* entries; // [T][k] logit of the entry, and 1 if it is the first of its column
+  float2* entries; // [T][k] logit of the entry, and 1 if it is the first (of lowest index) of its column
 };
 
 struct Sum {
@@ -154,6 +154,7 @@ void distill_kernel(const Args a) {
   extern __shared__ uint32_t bits[];  // a bit for every column of the piece: S; then the entries
   __shared__ float sh[2 * kWaves];
   __shared__ Teacher teacher;
+  __shared__ int twice;  // a column of the piece comes twice
   int* const s_idx = reinterpret_cast<int*>(bits + a.bit_words);  // column, < 0: padding
   int* const s_first = s_idx + a.k;
   float* const s_z = reinterpret_cast<float*>(s_first + a.k);
@@ -187,6 +188,7 @@ void distill_kernel(const Args a) {
   // ---- the teacher's entries
   if constexpr (kMode != kFinish)
     for (int i = tid; i < a.bit_words; i += kThreads) bits[i] = 0;
+  if (tid == 0) twice = 0;
   for (int i = tid; i < k; i += kThreads) {
     const int64_t o = row * a.ld_idx + i;
     const int64_t j = a.idx8 ? reinterpret_cast<const int64_t*>(a.idx)[o] : (int64_t)reinterpret_cast<const int32_t*>(a.idx)[o];
@@ -208,11 +210,26 @@ void distill_kernel(const Args a) {
       s_first[i] = 0;
       if (j < c0 || j >= c1) continue;
       const uint32_t bit = 1u << ((j - b0) & 31);
-      s_first[i] = !(atomicOr(&bits[(j - b0) >> 5], bit) & bit);  // one entry of a column is its first
+      s_first[i] = !(atomicOr(&bits[(j - b0) >> 5], bit) & bit);
+      if (!s_first[i]) twice = 1;
       s_z[i] = Elem<kT>::get(z[j]);
-      if constexpr (kMode == kStats) a.entries[row * k + i] = make_float2(s_z[i], (float)s_first[i]);
     }
     __syncthreads();
+    // Which of a column's entries came first is chance, and the order of S's sum with it: the first is that of lowest index.
+    if (twice) {
+      for (int i = tid; i < k; i += kThreads) {
+        const int j = s_idx[i];
+        if (j < c0 || j >= c1) continue;
+        int o = 0;
+        while (s_idx[o] != j) ++o;
+        s_first[i] = o == i;
+      }
+      __syncthreads();
+    }
+    if constexpr (kMode == kStats) {
+      for (int i = tid; i < k; i += kThreads)
+        if (s_idx[i] >= c0 && s_idx[i] < c1) a.entries[row * k + i] = make_float2(s_z[i], (float)s_first[i]);
+    }
   }
   if (kMode != kStats && tid < 64) {
     float tmax = kLowest, zm = kLowest, any = 0.f, dup = 0.f;
@@ -363,7 +380,7 @@ void distill_kernel(const Args a) {
       }
     }
     if (zero) return;
-    __syncthreads();  // this workgroup's stores have completed: S goes over them
+    __syncthreads();  // orders this workgroup's stores: S goes over them
     for (int i = tid; i < k; i += kThreads) {
       const int j = s_idx[i];
       if (j < c0 || j >= c1 || !s_first[i]) continue;
