@@ -166,12 +166,14 @@ __global__ __launch_bounds__(kThreads) void quant_kernel(const QuantArgs a) {
                       reinterpret_cast<const uint4*>(sttile)[tid - 64]);
 }
 
-// A workgroup takes 16 rows of four column tiles; thread t row t / 16 and columns 8 (t % 16) .. of each.
+// A workgroup takes 16 rows of four column tiles; thread t row t / 16 and columns 8 (t % 16) .. of each.  Row blocks past
+// what one grid dimension counts go on in the next.
 template <int kT, int kFmt>
 __global__ __launch_bounds__(kThreads) void dequant_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ s,
                                                            int64_t rows, int64_t cols, int64_t tiles, void* out, int vec) {
   typedef typename Elem<kT>::T T;
-  const int64_t r = (int64_t)blockIdx.y * 16 + (threadIdx.x >> 4);
+  const int64_t r0 = ((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * 16, r = r0 + (threadIdx.x >> 4);
+  if (r0 >= rows) return;
   const int cl = (threadIdx.x & 15) * 8;
   uint2 code[4];
   uint32_t e[4];
@@ -247,7 +249,8 @@ template <int kT>
 void launch_dequant(const void* q, const void* s, int64_t rows, int64_t cols, int64_t fmt, void* out, int vec,
                     hipStream_t st) {
   const int64_t tiles = (cols + 127) / 128;
-  const dim3 grid((unsigned)((tiles + 3) / 4), (unsigned)((rows + 15) / 16));
+  const int64_t blocks = (rows + 15) / 16, y = blocks < 65535 ? blocks : 65535;
+  const dim3 grid((unsigned)((tiles + 3) / 4), (unsigned)y, (unsigned)((blocks + y - 1) / y));
   if (fmt == MXFP4_E4M3)
     dequant_kernel<kT, MXFP4_E4M3><<<grid, kThreads, 0, st>>>((const uint8_t*)q, (const uint8_t*)s, rows, cols, tiles, out,
                                                               vec);
@@ -303,7 +306,7 @@ extern "C" int mxfp4_dequant(const void* q, const void* s, int64_t rows, int64_t
   MX_CHECK_ARG(q && s && out, "mxfp4_dequant: null pointer");
   MX_CHECK_ARG(mx_aligned(q, 16) && mx_aligned(s, 16) && mx_aligned(out, elem_size(type)),
                "mxfp4_dequant: misaligned buffer");
-  MX_CHECK_ARG((rows + 15) / 16 <= 65535 && cols < (1LL << 36), "mxfp4_dequant: too large");
+  MX_CHECK_ARG(rows < (1LL << 35) && cols < (1LL << 33), "mxfp4_dequant: too large");
   const int vec = mx_aligned(out, 16) && cols * elem_size(type) % 16 == 0;
   const hipStream_t hs = (hipStream_t)stream;
   if (type == MXFP4_BF16) launch_dequant<MXFP4_BF16>(q, s, rows, cols, fmt, out, vec, hs);
