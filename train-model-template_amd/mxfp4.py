@@ -14,6 +14,9 @@ that).  Everything runs in the hand-written kernels of libmxfp8_mlp.so; a CPU te
 Block scale: with amax the largest magnitude of the block and max = 6 (E2M1) or 448 (E4M3), the least power of two e with
 amax <= max e (so nothing is clipped), 2^-127 at the least; codes round to nearest, ties to even.  A NaN makes its block
 NaN; an infinity takes the format's largest value times 2^127.  Sums are fp32, with one rounding to the output's type.
+With act="e2m1" the products that they add are exact.  With act="e4m3" the matrix instruction adds groups of 16 in fewer
+bits: every term loses what lies below 2^-13 of the group's largest, 5e-6 of a result (rms) for normally distributed
+values and 7e-5 for values spread over a block's whole range, so some outputs round to a neighbour of what fp32 sums give.
 """
 import types
 
