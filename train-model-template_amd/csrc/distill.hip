@@ -394,6 +394,10 @@ void distill_kernel(const Args a) {
   }
 }
 
+// Threads a workgroup: of a whole row of nv vectors, and of a piece
+constexpr int64_t whole_threads(int64_t nv) { return nv <= 1024 ? 256 : nv <= 4096 ? 512 : 1024; }
+constexpr int kSplitThreads = 512;
+
 template <int kT>
 void launch(const Args& a0, int64_t T, int stages, hipStream_t st) {
   Args a = a0;
@@ -402,18 +406,18 @@ void launch(const Args& a0, int64_t T, int stages, hipStream_t st) {
   const size_t entries = (size_t)a.k * 16;
   if (stages == (DISTILL_STATS | DISTILL_FINISH) && a.parts == 1) {
     const size_t lds = a.bit_words * 4 + entries;
-    const int64_t nv = a.V / Vec<kT>::n;
-    if (nv <= 1024) distill_kernel<kT, kWhole, 256, 4><<<grid, 256, lds, st>>>(a);
-    else if (nv <= 4096) distill_kernel<kT, kWhole, 512, 8><<<grid, 512, lds, st>>>(a);
+    const int64_t nv = a.V / Vec<kT>::n, threads = whole_threads(nv);
+    if (threads == 256) distill_kernel<kT, kWhole, 256, 4><<<grid, 256, lds, st>>>(a);
+    else if (threads == 512) distill_kernel<kT, kWhole, 512, 8><<<grid, 512, lds, st>>>(a);
     else if (nv <= 8192) distill_kernel<kT, kWhole, 1024, 8><<<grid, 1024, lds, st>>>(a);
     else distill_kernel<kT, kWhole, 1024, 16><<<grid, 1024, lds, st>>>(a);
     return;
   }
-  if (stages & DISTILL_STATS) distill_kernel<kT, kStats, 512, 0><<<grid, 512, a.bit_words * 4 + entries, st>>>(a);
+  if (stages & DISTILL_STATS) distill_kernel<kT, kStats, kSplitThreads, 0><<<grid, kSplitThreads, a.bit_words * 4 + entries, st>>>(a);
   if (stages & DISTILL_FINISH) {
     a.wgs = a.grad ? a.parts : 1;
     a.bit_words = 0;
-    distill_kernel<kT, kFinish, 512, 0><<<(unsigned)(T * a.wgs), 512, entries, st>>>(a);
+    distill_kernel<kT, kFinish, kSplitThreads, 0><<<(unsigned)(T * a.wgs), kSplitThreads, entries, st>>>(a);
   }
 }
 
@@ -450,9 +454,9 @@ extern "C" int distill_topk_kl(const void* logits, int64_t type, int64_t ld, int
   MX_CHECK_ARG(tau > 0.f && tau < __builtin_inff(), "distill_topk_kl: the temperature has to be positive");
   MX_CHECK_ARG(parts >= 1 && parts <= DISTILL_MAX_PARTS && stages >= 1 && stages <= 3, "distill_topk_kl: bad plan");
   if (T == 0) return MXFP8_OK;
-  MX_CHECK_ARG(T < (1LL << 31) && T * parts * 1024 < (1LL << 32) * (V <= 4096 && parts == 1 ? 4 : 1),
-               "distill_topk_kl: more rows than one launch has threads for (T=%lld)", (long long)T);
   const bool whole = stages == 3 && parts == 1;
+  MX_CHECK_ARG(T < (1LL << 31) && T * parts * (whole ? whole_threads(V / (type == MXFP4_F32 ? 4 : 8)) : kSplitThreads) < (1LL << 32),
+               "distill_topk_kl: more rows than one launch has threads for (T=%lld)", (long long)T);
   MX_CHECK_ARG(logits && idx && t && (whole || ws) && (loss || grad || stages == DISTILL_STATS),
                "distill_topk_kl: null pointer");
   MX_CHECK_ARG(!grad || ld_grad >= V, "distill_topk_kl: bad gradient stride");
