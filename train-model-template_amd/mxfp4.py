@@ -88,6 +88,9 @@ class Weight:
     def __init__(self, w, transpose=True):
         self.handle = _native.host4().Weight(w, transpose)
 
+    def __deepcopy__(self, memo):
+        return self  # frozen: a copied model shares it
+
     @property
     def shape(self):
         return (self.handle.N, self.handle.K)
@@ -105,6 +108,9 @@ class GatedWeight:
 
     def __init__(self, w_gate, w_up):
         self.handle = _native.host4().Gated(w_gate, w_up)
+
+    def __deepcopy__(self, memo):
+        return self
 
     @property
     def shape(self):
