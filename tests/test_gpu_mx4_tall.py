@@ -17,7 +17,5 @@ def test_values_of_tall_matrices(gpu, R, fmt):
     step = 16 * 60000  # rows are quantized by themselves
     for r in range(0, R, step):
         assert torch.equal(v[r:r + step], mxfp4.mx4_dequant(mxfp4.mx4_quant(x[r:r + step], fmt=fmt), torch.bfloat16)), r
-    for rows in (x[:40], x[-40:]), (x[1048550:1048600],) * 2:
-        for part in rows:
-            lo = (part.data_ptr() - x.data_ptr()) // 64
-            assert torch.equal(v[lo:lo + len(part)].double().cpu(), mx4.values(part.cpu(), fmt))
+    for lo in (0, 1048448 - 20, 1048560 - 20, R - 40):  # the values themselves
+        assert torch.equal(v[lo:lo + 40].double().cpu(), mx4.values(x[lo:lo + 40].cpu(), fmt)), lo
