@@ -11,8 +11,8 @@
 // What bounds it: memory, the logits read once and the gradient written once.  A workgroup takes a row and holds it, or its
 // first 128K (64K in fp32) columns, in registers between the two passes; what is left comes from the cache the second time.
 // Few rows are split into pieces over two launches, joined by the second.  1000 rows of 65536 bf16 logits take 51 us (5.2
-// TB/s), 2048 of 248001 490 (4.1 TB/s counted once; 32K columns in registers and two workgroups a CU take the same); vectors
-// that begin 16-byte pieces but not lines took 505.  16 rows of 65536 fp32, the loss alone: 8.8 in the two launches.
+// TB/s), 2048 of 248001 478 (4.3 TB/s counted once; 32K columns in registers and two workgroups a CU take the same); vectors
+// that begin 16-byte pieces but not lines took 3% more.  16 rows of 65536 fp32, the loss alone: 9.0 in the two launches.
 #include <algorithm>
 
 #include "abi_common.h"

@@ -2,13 +2,14 @@
 // from fp32 into the operand of the product with [W_gate; W_up] (and, where an addend wants its gradient, rounded to the
 // activations' type).
 //
-// What bounds it: memory, 6 bytes read and 2 (E4M3) or 1 (E2M1) written for each column of a row, and 4 more for the addend's
-// gradient: 10752 x 6144 bf16 in E4M3 takes 90 us, 158 with the addend's gradient (5.9 and 5.0 TB/s; part of it comes from the
-// last-level cache); in pieces of 16 bytes of a row that gradient took 30 more.  The saved values lie in the order of the
-// forward epilogue's lanes, which is this kernel's order too: lane l of a wave holds row l % 32 and 16 columns of a 32 x 32
-// block, a 32-column scale block is two lanes, and every load of the saved values is 1 KB in a row.  One block a wave: four in
-// a row, each asked for while the one before was computed, took 98 us, and 11.7 where one takes 9.4 at 1000 x 3584, whose
-// waves then waited four times for memory.
+// What bounds it: memory, 6 bytes read and 2 (E4M3) or 1 (E2M1) written for each column of a row, and 4 more for the
+// addend's gradient: 10752 x 6144 bf16 in E4M3 takes 98 us, 159 with the addend's gradient (5.4 and 5.0 TB/s; part of it
+// comes from the last-level cache) in a training step, and 90 in a loop by itself; in pieces of 16 bytes of a row that
+// gradient took 30 more.  The saved values lie in the order of the forward epilogue's lanes, which is this kernel's order
+// too: lane l of a wave holds row l % 32 and 16 columns of a 32 x 32 block, a 32-column scale block is two lanes, and every
+// load of the saved values is 1 KB in a row.  One block a wave: four in a row, each asked for while the one before was
+// computed, took 98 us in that loop, and 11.7 where one takes 9.4 at 1000 x 3584, whose waves then waited four times for
+// memory.
 #include "abi_common.h"
 #include "mx4_device.h"
 

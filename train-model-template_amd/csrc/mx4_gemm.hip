@@ -10,11 +10,11 @@
 // The matrix instruction takes B's fragment first, so a lane's accumulators are one row m and, with B's rows in the PI
 // order, 16 contiguous columns.
 //
-// What bounds it.  Large products: in E4M3 the matrix pipe, busy 60-65% of cycles at a clock that the power limit holds at
-// 1.9 GHz (10752 x 2048 x 12288 205 us, 2.6 PFLOP/s); in E2M1, at 3.5-3.7 PFLOP/s (10752 x 2048 x 6144 73-77 us, x 6144 x 2048
-// 77-82), the pipe is busy 38-44% at 2.0 GHz and no other unit more (LDS 17-20%, reads of 340 cycles, 82% of them from L2):
-// waves wait to issue, and a tile's fill and epilogue are 3 of its 10 us at K = 2048.  Small ones: the chain of a tile's K
-// tiles, 0.10 (E2M1) to 0.15 us (E4M3) each.
+// What bounds it (times from kernel traces of whole training steps, from box to box).  Large products: in E4M3 the matrix
+// pipe, busy 59-64% of cycles at a clock that the power limit holds at 1.9 GHz (10752 x 2048 x 12288 228-245 us, 2.2-2.4
+// PFLOP/s); in E2M1, at 3.0-3.5 PFLOP/s (10752 x 2048 x 6144 77-80 us, x 6144 x 2048 85-90), the pipe is busy 36-44% at 2.0 GHz
+// and no other unit more (LDS 17-20%, reads of 340 cycles, 80% of them from L2): waves wait to issue, and a tile's fill and
+// epilogue are 3 of its 10 us at K = 2048.  Small ones: the chain of a tile's K tiles, 0.10 (E2M1) to 0.15 us (E4M3) each.
 #include <algorithm>
 #include <type_traits>
 
@@ -456,7 +456,7 @@ void gemm_kernel(const GemmArgs g) {
 
 // Every ring leaves room for two workgroups a CU, so that one's pipeline fill, barriers and epilogue overlap the other's
 // products: 256 x 256 tiles with one took 87 us (E2M1, 10752 x 6144 x 2048) and 148 (10752 x 2048 x 12288) where these take 78
-// and 128.  In Tall the E4M3 stages are 64 codes wide, the E2M1 ones 128 (half the barriers).  The others hold a whole K
+// and 128, each product in a loop by itself.  In Tall the E4M3 stages are 64 codes wide, the E2M1 ones 128 (half the barriers).  The others hold a whole K
 // tile's fragments ahead, for which Tall has no registers left: at 1000 x 1024 x 7168 in E4M3 that took Low from 16.3 to 14.2
 // us, Mid from 22.0 to 20.4, and Mini (twice Low's workgroups where those leave CUs idle) from 14.6 to 13.6.
 template <int kAF>

@@ -1,9 +1,9 @@
 // MX quantization to E2M1 (or E4M3) operands of the 4-bit products, along the rows and, from the same read, along the
 // columns; and the values of an operand.
 //
-// What bounds it: memory.  A bf16 element is read once (2 bytes) and leaves as 17/32 byte an axis (E2M1): [10752, 6144] takes 36
-// us (4.6 TB/s), [10752, 2048] 15.6 (3.6 TB/s; 12.9 at the rate of a large copy in E4M3), both axes of [6144, 2048] 10.8;
-// small matrices a launch and one round trip, 5 us.
+// What bounds it: memory.  A bf16 element is read once (2 bytes) and leaves as 17/32 byte an axis (E2M1): in a training step
+// [10752, 6144] takes 37 us (4.5 TB/s; 26 where the last-level cache holds the matrix), [10752, 2048] 16 (3.5 TB/s), 15 to 16 in
+// E4M3 (12.9 at the rate of a large copy), both axes of [6144, 2048] 10.7; small matrices a launch and one round trip, 5 us.
 // One 256-thread workgroup per 128 x 128 tile, which is one 512-byte scale tile of either axis: lane l of wave w (rg =
 // l / 16, ch = l % 16) holds columns 8 ch .. + 7 of rows 32 w + 8 rg + 0..7, so a 32-column block of a row is four
 // neighbouring lanes and a 32-row block of a column is one wave.
