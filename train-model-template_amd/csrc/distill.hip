@@ -7,6 +7,8 @@
 // fp32 over the columns outside S (a bit for every column in LDS says which), and S is added from its k values: q_r has its
 // own maximum and sum and is no difference.  The factors exp((m - M) / tau) / sum and p_r / s that the gradient needs are at
 // most 1 each.  z - m is taken before the division by tau: rows of the type's lowest value stay uniform.
+// The loss sums logarithms and differences of logits apart, tau (tau l + d): a difference that reaches the type's end is not
+// divided by tau.
 //
 // What bounds it: memory, the logits read once and the gradient written once.  A workgroup takes a row and holds it, or its
 // first 128K (64K in fp32) columns, in registers between the two passes; what is left comes from the cache the second time.
@@ -139,7 +141,8 @@ struct Teacher {
   float psum;    // sum of p
   float rest;    // p_r
   float zm, own; // maximum and sum of exp((z - zm) / tau) over S
-  float a;       // sum of p (log p - (z - zm) / tau)
+  float a;       // sum of p log p
+  float b;       // sum of p (z - zm)
   float dup;     // a column comes twice
 };
 
@@ -246,7 +249,7 @@ void distill_kernel(const Args a) {
     zm = wave_max(zm);
     dup = wave_max(dup);
     const float lse = a.lse ? a.lse[row] : 0.f;
-    float psum = 0.f, own = 0.f, A = 0.f;
+    float psum = 0.f, own = 0.f, A = 0.f, B = 0.f;
     for (int i = tid; i < k; i += 64)
       if (s_idx[i] >= 0) {
         psum += a.lse ? expf(s_p[i] * itau - lse) : expf((s_p[i] - tmax) * itau);
@@ -260,10 +263,14 @@ void distill_kernel(const Args a) {
         const float logp = a.lse ? s_p[i] * itau - lse : (s_p[i] - tmax) * itau - norm;
         const float p = expf(logp);
         s_p[i] = p;
-        if (p > 0.f || p != p) A += p * (logp - (s_z[i] - zm) * itau);
+        if (p > 0.f || p != p) {
+          A += p * logp;
+          B += p * (s_z[i] - zm);
+        }
       }
     A = wave_sum(A);
-    if (tid == 0) teacher = Teacher{any, a.lse ? psum : 1.f, a.lse ? fmaxf(1.f - psum, 0.f) : 0.f, zm, own, A, dup};
+    B = wave_sum(B);
+    if (tid == 0) teacher = Teacher{any, a.lse ? psum : 1.f, a.lse ? fmaxf(1.f - psum, 0.f) : 0.f, zm, own, A, B, dup};
   }
 
   // ---- the running maximum and sum outside S
@@ -335,9 +342,12 @@ void distill_kernel(const Args a) {
     const float rest = tot.s == 0.f && tc.rest < 0x1p-16f ? 0.f : tc.rest;
     if (a.loss && first && tid == 0) {
       const float log_total = total == 0.f ? 0.f : logf(total);
-      float l = tc.a + tc.psum * ((big - tc.zm) * itau + log_total);
-      if (rest > 0.f) l += rest * (logf(rest) - ((tot.m - big) * itau + logf(tot.s) - log_total));
-      a.loss[row] = live ? l * a.tau * a.tau : 0.f;
+      float l = tc.a + tc.psum * log_total, d = tc.psum * (big - tc.zm) - tc.b;
+      if (rest > 0.f) {
+        l += rest * (logf(rest) - logf(tot.s) + log_total);
+        d += rest * (big - tot.m);
+      }
+      a.loss[row] = live ? a.tau * (a.tau * l + d) : 0.f;
     }
     if (!a.grad) return;
     const bool zero = !live || weight == 0.f || total == 0.f;
